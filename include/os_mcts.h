@@ -358,6 +358,104 @@ int os_az_mlp_heads_async(const float* obs, int64_t num_rows, int32_t obs_size,
                           int32_t num_actions, const uint8_t* legal, double* prior,
                           double* value, void* hip_stream);
 
+/* ---- Policy operators ---------------------------------------------------
+ * What a program that trains on, or reports, a network's policy does with its
+ * logits beside the search (os_az_heads_async turns the same rows into priors
+ * and values).  Row r holds num_actions logits at logits + r * ld elements
+ * (ld may be 0: one row for all); legal[r * legal_ld + a] == 0 excludes an
+ * action (legal NULL: none is; legal_ld may be 0).  A logit of -inf excludes
+ * its action too.  With x = logit / temperature on the remaining actions,
+ * p = softmax(x).  A row without any is empty: p = 0, gradient 0.  A NaN or
+ * +inf logit on a legal action makes its row's results NaN and no other row's.
+ * Logits f32, bf16 or f16 (dtype); arithmetic and results f32; gradients are
+ * rounded once to the logits' type.  Buffers do not overlap.  Every call
+ * launches on hip_stream, whose device must be current, allocates nothing and
+ * may be captured; it reads no device data on the host, so what ids hold is
+ * checked on the device, as said with each. */
+#define OS_AZ_F32 0
+#define OS_AZ_BF16 1
+#define OS_AZ_F16 2
+#define OS_AZ_MAX_ACTIONS 4194304
+#define OS_AZ_MAX_TOP 64
+#define OS_AZ_MAX_TARGETS 1024
+typedef struct os_az_rows {
+  const void* logits;
+  const uint8_t* legal; /* NULL: every action */
+  int64_t num_rows;
+  int64_t ld;           /* logits row stride, elements */
+  int64_t legal_ld;     /* legal row stride, bytes */
+  int32_t num_actions;  /* 1 .. OS_AZ_MAX_ACTIONS */
+  int32_t dtype;        /* OS_AZ_F32 / _BF16 / _F16 */
+  float temperature;    /* > 0, finite */
+  int32_t reserved;     /* 0 */
+} os_az_rows;
+/* A target distribution on k listed actions of each row: entry j of row r is
+ * action actions[r * actions_ld + j] (int32, or int64 when wide) with the value
+ * target[r * target_ld + j].  Negative actions are padding.  An action listed
+ * twice counts twice.  Value types: teacher logits z (f32 / bf16 / f16;
+ * q = softmax(z / temperature) over the row's entries, -inf: no mass), or
+ * weights (f32 / int32, q = w / sum w, those not above 0 count as 0: a search's
+ * visit counts).  actions NULL with k = num_actions: entry j is action j. */
+#define OS_AZ_LOGITS_F32 0
+#define OS_AZ_LOGITS_BF16 1
+#define OS_AZ_LOGITS_F16 2
+#define OS_AZ_WEIGHTS_F32 3
+#define OS_AZ_WEIGHTS_I32 4
+typedef struct os_az_target {
+  const void* actions;
+  const void* target;
+  int64_t actions_ld;
+  int64_t target_ld;
+  int32_t k;            /* 0 .. OS_AZ_MAX_TARGETS */
+  int32_t type;
+  int32_t wide;         /* actions are int64 */
+  int32_t reserved;     /* 0 */
+} os_az_target;
+/* Bytes of device workspace os_az_logprobs_async (top alternatives) or
+ * os_az_distill_async (top = 0) needs for these rows (0: none, pass NULL);
+ * not initialised, free again once the call's work on the stream is done.
+ * < 0: the error of the call itself. */
+int64_t os_az_rows_workspace(const os_az_rows* rows, int32_t top);
+/* logprob[r] = log p[actions[r]] (0 for a negative action, -inf for one that is
+ * excluded, NaN for one >= num_actions), entropy[r] = -sum p log p, and the
+ * `top` most likely actions (ties to the lowest) with their log probabilities,
+ * in top_action / top_logprob [num_rows][top]; past the row's actions, and in a
+ * NaN row, -1 with -inf / NaN.  stats[num_rows][2], for the gradient: the row's
+ * maximal logit and log2 of its exponentials' sum (0, 0: empty row).  actions
+ * and logprob may both be NULL, stats too, the top pair when top = 0. */
+int os_az_logprobs_async(const os_az_rows* rows, const void* actions, int32_t wide,
+                             float* logprob, float* entropy, float* stats, int32_t top,
+                             int64_t* top_action, float* top_logprob, void* workspace,
+                             int64_t workspace_bytes, void* hip_stream);
+/* Its gradient: grad[r * grad_ld + i] = d(sum_r g_logprob[r] logprob[r] +
+ * g_entropy[r] entropy[r] + sum_k g_top[r][k] top_logprob[r][k]) / d logits[r][i],
+ * 0 where the action is excluded.  g_logprob / g_entropy have element strides of
+ * their own (0: one value for all rows); NULL: no such term.  stats and
+ * entropy as os_az_logprobs_async left them.  An action that is negative
+ * has no term, one >= num_actions makes its row NaN. */
+int os_az_logprobs_grad_async(const os_az_rows* rows, const void* actions, int32_t wide,
+                                  const float* entropy, const float* stats, int32_t top,
+                                  const int64_t* top_action, const float* g_logprob,
+                                  int64_t g_logprob_stride, const float* g_entropy,
+                                  int64_t g_entropy_stride, const float* g_top, void* grad,
+                                  int64_t grad_ld, void* hip_stream);
+/* loss[r] = -sum_j q_j log p[a_j], the cross entropy (+inf when an excluded
+ * action has mass, NaN when a listed action is >= num_actions; 0 when the row
+ * has no target), target_entropy[r] = -sum_j q_j log q_j (loss - target_entropy
+ * is the Kullback-Leibler divergence; NULL: not wanted), stats as above (NULL:
+ * not wanted).  grad != NULL: grad[r][i] = weight[r] d loss[r] / d logits[r][i]
+ * = weight[r] (p_i sum q - q_i) / temperature, 0 where the action is excluded;
+ * weight NULL: 1. */
+int os_az_distill_async(const os_az_rows* rows, const os_az_target* target,
+                            const float* weight, float* loss, float* target_entropy,
+                            float* stats, void* grad, int64_t grad_ld, void* workspace,
+                            int64_t workspace_bytes, void* hip_stream);
+/* The gradient alone, from the stats os_az_distill_async left: weight has an
+ * element stride (0: one value for all rows). */
+int os_az_distill_grad_async(const os_az_rows* rows, const os_az_target* target,
+                                 const float* weight, int64_t weight_stride, const float* stats,
+                                 void* grad, int64_t grad_ld, void* hip_stream);
+
 /* ---- Self-play -----------------------------------
  * num_games independent games, each played on the device the way
  * examples/mcts_example.cc:77-136 PlayGame drives two MCTSBots sharing ONE
@@ -513,7 +611,7 @@ int64_t os_make_roots(const os_game* game, int64_t num_roots, uint32_t seed_base
 int32_t os_sample_action(const double* probs, int32_t n, uint32_t* key, int32_t* pos);
 
 /* sizeof of the named ABI struct ("os_mcts_params", "os_game_info",
- * "os_selfplay_options") as this library was built, or OS_ERR_INVALID for an
+ * "os_selfplay_options", "os_az_rows", "os_az_target") as this library was built, or OS_ERR_INVALID for an
  * unknown name: lets a binding (ctypes, cgo, JNI) check its own layout once at
  * load time.  No reference counterpart (pybind11 checks types at compile
  * time, pyspiel.cc:499-524). */

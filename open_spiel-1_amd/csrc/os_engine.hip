@@ -1196,6 +1196,8 @@ int64_t os_abi_struct_size(const char* name) {
   if (n == "os_mcts_params") return sizeof(os_mcts_params);
   if (n == "os_game_info") return sizeof(os_game_info);
   if (n == "os_selfplay_options") return sizeof(os_selfplay_options);
+  if (n == "os_az_rows") return sizeof(os_az_rows);
+  if (n == "os_az_target") return sizeof(os_az_target);
   return Fail(OS_ERR_INVALID, "unknown ABI struct " + n);
 }
 

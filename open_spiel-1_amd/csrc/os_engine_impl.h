@@ -17,19 +17,13 @@
 
 #include "../../include/os_mcts.h"
 #include "os_az.h"
+#include "os_error.h"
 #include "os_host.h"
 #include "os_mcts.h"
 #include "os_wave.h"
 
 namespace osx {
 using namespace osm;
-
-// Thread-local message of the last failed C-ABI call (os_last_error).
-extern thread_local std::string g_err;
-inline int Fail(int code, const std::string& msg) {
-  g_err = msg;
-  return code;
-}
 
 // Host-side per-root work (root replay, Dirichlet draws) over [0, n) in
 // contiguous chunks on up to 16 threads, the calling thread taking the first.
@@ -55,13 +49,6 @@ int ParallelChunks(int64_t n, int64_t min_chunk, F body) {
     if (rc[t]) return Fail(rc[t], msg[t]);
   return 0;
 }
-#define HIP_TRY(expr)                                                        \
-  do {                                                                       \
-    hipError_t _e = (expr);                                                  \
-    if (_e != hipSuccess)                                                    \
-      return ::osx::Fail(OS_ERR_DEVICE, std::string(#expr " failed: ") +    \
-                                            hipGetErrorString(_e));          \
-  } while (0)
 
 constexpr int kGoLogCap = 248;              // >= 2 * 11 * 11 + 4
 constexpr int kGoHeads = 122;               // stone counts 0 .. 11 * 11

@@ -6,6 +6,8 @@ Submodules:
            (the `pyspiel` surface the Python bot path uses)
   mcts     Evaluator / RandomRolloutEvaluator / SearchNode / MCTSBot
            (open_spiel/python/algorithms/mcts.py drop-in)
+  policy   policy operators on a network's logits: log probabilities with
+           entropy and top actions, distillation (with gradients)
   dist     multi-GPU sharding (torch.distributed / RCCL)
 """
 from . import _lib  # noqa: F401  (fails loudly if libos_mcts.so is missing)

@@ -84,6 +84,18 @@ class MctsParams(ctypes.Structure):
               ("child_selection", _i32), ("reserved", _i32)]
 
 
+class AzRows(ctypes.Structure):
+  _fields_ = [("logits", ctypes.c_void_p), ("legal", ctypes.c_void_p), ("num_rows", _i64),
+              ("ld", _i64), ("legal_ld", _i64), ("num_actions", _i32), ("dtype", _i32),
+              ("temperature", ctypes.c_float), ("reserved", _i32)]
+
+
+class AzTarget(ctypes.Structure):
+  _fields_ = [("actions", ctypes.c_void_p), ("target", ctypes.c_void_p), ("actions_ld", _i64),
+              ("target_ld", _i64), ("k", _i32), ("type", _i32), ("wide", _i32),
+              ("reserved", _i32)]
+
+
 def _sig(name, restype, argtypes):
   f = getattr(lib, name)
   f.restype = restype
@@ -190,6 +202,19 @@ _sig("os_az_prepare_staged", ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp])
 _sig("os_az_set_noise", ctypes.c_int, [_vp, _P, _i64, ctypes.c_double])
 _sig("os_az_tree_priors", ctypes.c_int, [_vp, _i64, _i64, _P])
 AZ_REQUESTS_SEPARATE, AZ_REQUESTS_FUSED = 0, 1
+_rows_p, _target_p = ctypes.POINTER(AzRows), ctypes.POINTER(AzTarget)
+_sig("os_az_rows_workspace", _i64, [_rows_p, _i32])
+_sig("os_az_logprobs_async", ctypes.c_int,
+     [_rows_p, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp])
+_sig("os_az_logprobs_grad_async", ctypes.c_int,
+     [_rows_p, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp])
+_sig("os_az_distill_async", ctypes.c_int,
+     [_rows_p, _target_p, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp])
+_sig("os_az_distill_grad_async", ctypes.c_int,
+     [_rows_p, _target_p, _vp, _i64, _vp, _vp, _i64, _vp])
+AZ_F32, AZ_BF16, AZ_F16 = 0, 1, 2
+AZ_LOGITS_F32, AZ_LOGITS_BF16, AZ_LOGITS_F16, AZ_WEIGHTS_F32, AZ_WEIGHTS_I32 = range(5)
+AZ_MAX_ACTIONS, AZ_MAX_TOP, AZ_MAX_TARGETS = 4194304, 64, 1024
 _sig("os_az_fetch", ctypes.c_int, [_vp, _i32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P])
 _sig("os_engine_node_bytes", _i32, [_vp])
 _sig("os_engine_state_bytes", _i32, [_vp])
@@ -201,7 +226,8 @@ def _check_abi_layout():
   """The library reports the struct sizes it was built with: a stale build or
   binding fails at import instead of misreading parameters."""
   for name, cls in (("os_mcts_params", MctsParams), ("os_game_info", GameInfo),
-                    ("os_selfplay_options", SelfPlayOptions)):
+                    ("os_selfplay_options", SelfPlayOptions), ("os_az_rows", AzRows),
+                    ("os_az_target", AzTarget)):
     n = lib.os_abi_struct_size(name.encode())
     if n != ctypes.sizeof(cls):
       raise ImportError("%s: libos_mcts.so has %d bytes, the ctypes binding %d "
