@@ -1,0 +1,1317 @@
+// Policy operators on a network's logits rows (include/os_mcts.h, "Policy
+// operators"): log probabilities with entropy and top actions, distillation
+// from listed targets, and their gradients.  Kernels; os_policy.hip checks the
+// arguments and chooses among them, os_policy_{f32,bf16,f16}.hip instantiate
+// them, one unit a type so that they build in parallel.
+//
+// Mathematics.  With c = log2(e) / temperature, m the row's maximal logit on an
+// allowed action and l = log2 sum_i 2^((x_i - m) c), everything follows from
+// (m, l): log2 p_i = (x_i - m) c - l, and with d_i = (x_i - m) c, e_i = 2^d_i
+// the entropy is ln 2 (l - sum e_i d_i / sum e_i).  An excluded action is
+// x_i = -inf, e_i = 0.  The difference is taken before the scaling, so rows of
+// the type's lowest value, or with a large common offset, lose nothing; sums
+// are held in float32, at most 128 terms a lane, then joined in trees.
+//
+// What bounds it.  Two to four bytes an element against one exponential and
+// some eight other operations (two exponentials with the gradient): HBM, when
+// the card is full, with the vector units about half busy - so each row is read
+// ONCE, by whole workgroups, and stays in registers (16 chunks of 16 bytes a
+// lane: up to 256 KiB a workgroup, the register file being 512 KiB a compute
+// unit) from the sums to the gradient or the selection of the top actions.
+// The maximum and the sums run together over the chunks as they arrive (a
+// running maximum, the sums rescaled by it), and a chunk's registers are
+// reloaded with the next row's data as soon as the last pass is through with
+// them, so the loads of row r + 1 run under the arithmetic of row r.
+#ifndef OS_POLICY_H_
+#define OS_POLICY_H_
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/os_mcts.h"
+
+namespace osp {
+
+constexpr float kLn2 = 0.69314718055994530942f;
+// d below this is e = 0 in f32 (2^-149 is the least subnormal): keeps 0 * -inf
+// out of the sums.
+constexpr float kFloor = -160.0f;
+// The running maximum's start: finite, so that (-inf) - m is never NaN.
+constexpr float kLowest = -3.4028234663852886e38f;
+constexpr int kTinyMax = 64;       // rows of up to this many actions: 16 lanes each
+constexpr int kMaxWaves = 16;
+constexpr int kMaxSplit = 64;      // parts of a row
+constexpr int kCandidates = 512;   // top actions: LDS list
+constexpr int kFewChunks = 4;      // chunks a lane in the kernels for short rows
+constexpr int kChunks = 16;        // for long ones
+constexpr int kMaskChunks = 8;     // with a mask
+
+struct Rows {
+  const void* x;
+  const uint8_t* legal;
+  int64_t n, ld, lld;
+  int32_t v;
+  float c;      // log2(e) / temperature
+  float inv_t;  // 1 / temperature
+};
+
+struct Target {
+  const void* ids;
+  const void* val;
+  int64_t ids_ld, val_ld;
+  int32_t k, type, wide;
+};
+
+// How the workgroups share the rows: blockIdx.y is a part of a row, `part`
+// actions long (a multiple of 64; the last part is shorter, never below 64
+// where there are several), blockIdx.x strides over the rows.
+struct Parts {
+  int32_t parts, part;
+};
+
+// One part's sums, for k_join; its top keys follow in a list of their own.
+struct PartSums {
+  float m, s, t, pad;
+};
+
+struct LogprobArgs {
+  const void* actions;
+  int32_t wide, top;
+  float* logprob;
+  float* entropy;
+  float* stats;
+  int64_t* top_action;
+  float* top_logprob;
+  PartSums* sums;      // != nullptr: write parts, not results
+  uint64_t* part_keys;
+};
+
+struct LogprobGradArgs {
+  const void* actions;
+  int32_t wide, top;
+  const float* entropy;
+  const float* stats;
+  const int64_t* top_action;
+  const float* gl;
+  int64_t gls;
+  const float* gh;
+  int64_t ghs;
+  const float* gt;
+  void* grad;
+  int64_t grad_ld;
+};
+
+struct DistillArgs {
+  Target t;
+  const float* weight;
+  int64_t weight_stride;
+  float* loss;
+  float* tent;
+  float* stats;  // kDistillGrad reads them
+  void* grad;
+  int64_t grad_ld;
+  int32_t hash;  // LDS table entries (a power of two)
+};
+
+struct JoinArgs {
+  LogprobArgs lp;
+  DistillArgs ds;
+  int32_t parts;
+};
+
+enum Op : int { kLogprobs, kLogprobsTop, kLogprobsGrad, kDistill, kDistillFused, kDistillGrad };
+
+// The compiler must take x for a new value: it would otherwise keep what was
+// computed from it earlier (every chunk's converted elements, every offset) in
+// registers that the rows need.  No instruction.
+template <class V>
+__device__ __forceinline__ void renew(V& x) {
+  asm volatile("" : "+v"(x));
+}
+
+__device__ __forceinline__ float neg_inf() { return -__builtin_huge_valf(); }
+__device__ __forceinline__ float exp2_(float d) { return __builtin_amdgcn_exp2f(d); }
+
+// ---- element types ----
+
+template <class T>
+constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // elements of a 16-byte chunk
+
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using f32x2 = __attribute__((ext_vector_type(2))) float;
+
+__device__ __forceinline__ float get(const float* p, int64_t i) { return p[i]; }
+__device__ __forceinline__ float get(const __bf16* p, int64_t i) { return static_cast<float>(p[i]); }
+__device__ __forceinline__ float get(const _Float16* p, int64_t i) { return static_cast<float>(p[i]); }
+
+// Rows start anywhere their type may (an odd row stride, a view's column
+// offset): wide accesses are declared with the element's alignment only.
+template <class T, class W>
+__device__ __forceinline__ W load_at(const T* p) {
+  struct __attribute__((packed, aligned(sizeof(T)))) P { W w; };
+  return reinterpret_cast<const P*>(p)->w;
+}
+template <class T, class W>
+__device__ __forceinline__ void store_at(T* p, W w) {
+  struct __attribute__((packed, aligned(sizeof(T)))) P { W w; };
+  reinterpret_cast<P*>(p)->w = w;
+}
+
+template <class T>
+__device__ __forceinline__ void unpack(u32x4 r, float (&x)[kPer<T>]) {
+  if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(r[j]);
+  } else if constexpr (std::is_same_v<T, __bf16>) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = __uint_as_float(r[j] << 16);
+      x[2 * j + 1] = __uint_as_float(r[j] & 0xFFFF0000u);
+    }
+  } else {
+    using h2 = __attribute__((ext_vector_type(2))) _Float16;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const h2 h = __builtin_bit_cast(h2, static_cast<uint32_t>(r[j]));
+      x[2 * j] = static_cast<float>(h[0]);
+      x[2 * j + 1] = static_cast<float>(h[1]);
+    }
+  }
+}
+// Round to nearest even, once.
+template <class T>
+__device__ __forceinline__ u32x4 pack(const float (&x)[kPer<T>]) {
+  u32x4 r;
+  if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = __float_as_uint(x[j]);
+  } else {
+    using h2 = __attribute__((ext_vector_type(2))) T;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 f = {x[2 * j], x[2 * j + 1]};
+      r[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, h2));
+    }
+  }
+  return r;
+}
+
+__device__ __forceinline__ int64_t get_id(const void* p, int wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+}
+
+// One element of row r (-inf: excluded).
+template <class T>
+__device__ __forceinline__ float logit(const Rows& a, int64_t r, int64_t i) {
+  const float x = get(static_cast<const T*>(a.x) + r * a.ld, i);
+  return a.legal != nullptr && a.legal[r * a.lld + i] == 0 ? neg_inf() : x;
+}
+
+// ln p of a logit: right for any x of the type ((x - m) c may overflow).
+__device__ __forceinline__ float log_p(const Rows& a, float x, float m, float l) {
+  return fmaf(x - m, a.inv_t, -l * kLn2);
+}
+
+// ---- reductions ----
+
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xF, 0xF, true));
+}
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, 0xF, 0xF, true));
+}
+struct Add {
+  __device__ float operator()(float a, float b) const { return a + b; }
+};
+struct Max {
+  __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct MinU {
+  __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return a < b ? a : b; }
+};
+// Over each 16 lanes (pairs, quads, then mirrored halves): all of them get it.
+template <class T, class F>
+__device__ __forceinline__ T fold16(T v, F f) {
+  v = f(v, dpp<0xB1>(v));
+  v = f(v, dpp<0x4E>(v));
+  v = f(v, dpp<0x141>(v));
+  return f(v, dpp<0x140>(v));
+}
+__device__ __forceinline__ float lane_at(float v, int i) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
+}
+template <class F>
+__device__ __forceinline__ float fold64(float v, F f) {
+  v = fold16(v, f);
+  return f(f(lane_at(v, 0), lane_at(v, 16)), f(lane_at(v, 32), lane_at(v, 48)));
+}
+
+// Sums relative to a maximum: s = sum 2^((x - m) c), t = sum (..)(x - m) c.
+struct Sums {
+  float m, s, t;
+};
+template <bool kEnt>
+__device__ __forceinline__ Sums fold_sums(Sums a, float c) {
+  const float m = fold64(a.m, Max{});
+  const float d = (a.m - m) * c;
+  const float f = exp2_(d);
+  Sums r;
+  r.m = m;
+  r.s = fold64(a.s * f, Add{});
+  r.t = kEnt ? fold64(f * fmaf(a.s, fmaxf(d, kFloor), a.t), Add{}) : 0.0f;
+  return r;
+}
+
+// A target's unnormalised value (weights: those not above 0 are no mass, -inf)
+// and its mass relative to the row's largest.
+__device__ __forceinline__ float target_value(const Target& t, int64_t i) {
+  float z;
+  switch (t.type) {
+    case OS_AZ_LOGITS_F32: return static_cast<const float*>(t.val)[i];
+    case OS_AZ_LOGITS_BF16: return get(static_cast<const __bf16*>(t.val), i);
+    case OS_AZ_LOGITS_F16: return get(static_cast<const _Float16*>(t.val), i);
+    case OS_AZ_WEIGHTS_F32: z = static_cast<const float*>(t.val)[i]; break;
+    default: z = static_cast<float>(static_cast<const int32_t*>(t.val)[i]); break;
+  }
+  return z <= 0.0f ? neg_inf() : z;
+}
+__device__ __forceinline__ float target_mass(const Target& t, float c, float z, float ref) {
+  if (z == neg_inf()) return 0.0f;
+  return t.type >= OS_AZ_WEIGHTS_F32 ? z / ref : exp2f((z - ref) * c);
+}
+// Entry j of a row: its action (< 0: none) and value.
+struct Entry {
+  int64_t id;
+  float z;
+};
+__device__ __forceinline__ Entry target_entry(const Target& t, int64_t r, int j) {
+  Entry e;
+  e.id = t.ids != nullptr ? get_id(t.ids, t.wide, r * t.ids_ld + j) : j;
+  e.z = e.id < 0 ? neg_inf() : target_value(t, r * t.val_ld + j);
+  return e;
+}
+// Running (maximum, mass relative to it) of target entries.
+struct Mass {
+  float z, s;
+};
+__device__ __forceinline__ void mass_add(const Target& t, float c, float z, Mass& a) {
+  if (z > a.z) {
+    a.s = a.s * target_mass(t, c, a.z, z) + 1.0f;
+    a.z = z;
+  } else if (z != neg_inf()) {
+    a.s += target_mass(t, c, z, a.z);
+  }
+}
+template <class MaxF, class AddF>
+__device__ __forceinline__ Mass mass_fold(const Target& t, float c, Mass a, MaxF maxf, AddF addf) {
+  const float z = maxf(a.z);
+  return Mass{z, addf(a.s * target_mass(t, c, a.z, z))};
+}
+
+// ---- top actions ----
+
+// A larger value first, of equal ones the lower index, as unsigned integers; 0
+// is no key.
+__device__ __forceinline__ uint64_t top_key(float x, uint32_t i) {
+  uint32_t u = __float_as_uint(x + 0.0f);  // -0 and +0 are equal
+  u = (u >> 31) ? ~u : (u | 0x80000000u);
+  return (static_cast<uint64_t>(u) << 32) | (0xFFFFFFFFu - i);
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t u = static_cast<uint32_t>(k >> 32);
+  return __uint_as_float((u >> 31) ? (u & 0x7FFFFFFFu) : ~u);
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t k) {
+  return 0xFFFFFFFFu - static_cast<uint32_t>(k);
+}
+__device__ __forceinline__ uint64_t fold64_max(uint64_t v) {
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t q = __shfl_xor(v, o);
+    v = q > v ? q : v;
+  }
+  return v;
+}
+// The k-th largest (k >= 1) of one key a lane.
+__device__ __forceinline__ uint64_t kth64(uint64_t key, int k) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t lo = static_cast<uint32_t>(key), hi = static_cast<uint32_t>(key >> 32);
+  int rank = 0;
+#pragma unroll 8
+  for (int j = 0; j < 64; ++j) {
+    const uint64_t q =
+        (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(hi), j))) << 32) |
+        static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(lo), j));
+    rank += q > key || (q == key && j < lane) ? 1 : 0;
+  }
+  const uint64_t at = __ballot(rank == k - 1);
+  const int src = __builtin_ctzll(at);
+  return (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(hi), src))) << 32) |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(lo), src));
+}
+
+struct TopLds {
+  uint64_t group[64];  // largest key of lane i of every wave
+  uint64_t limit;
+  uint32_t count;
+  uint64_t cand[kCandidates];
+};
+
+// ---- the listed entries of a gradient ----
+
+// A row's listed actions in an open-addressed LDS table: key (action, -1:
+// free), the weight to add there and its logit.  Distinct actions are inserted
+// in parallel; where one is met twice, `twice` is set and one lane rebuilds the
+// table in list order, so a sum never depends on the order of waves.
+struct Table {
+  int32_t* key;
+  float* w;
+  float* x;
+  int32_t mask;
+};
+__device__ __forceinline__ uint32_t table_slot(const Table& t, int32_t id) {
+  return (static_cast<uint32_t>(id) * 2654435761u >> 16) & t.mask;
+}
+__device__ __forceinline__ void table_clear(const Table& t, int tid, int step) {
+  for (int i = tid; i <= t.mask; i += step) t.key[i] = -1;
+}
+__device__ __forceinline__ bool table_put(const Table& t, int32_t id, float w, float x) {
+  uint32_t s = table_slot(t, id);
+  for (;;) {  // (at most half full: a free slot is met)
+    const int32_t old = atomicCAS(&t.key[s], -1, id);
+    if (old == -1) {
+      t.w[s] = w;
+      t.x[s] = x;
+      return true;
+    }
+    if (old == id) return false;
+    s = (s + 1) & t.mask;
+  }
+}
+// One lane alone: adds to what is there.
+__device__ __forceinline__ void table_add(const Table& t, int32_t id, float w, float x) {
+  uint32_t s = table_slot(t, id);
+  while (t.key[s] != -1 && t.key[s] != id) s = (s + 1) & t.mask;
+  if (t.key[s] == id) {
+    t.w[s] += w;
+  } else {
+    t.key[s] = id;
+    t.w[s] = w;
+    t.x[s] = x;
+  }
+}
+
+// p_i (f0 + f1 ln p_i) of a logit.
+struct Dense {
+  float m, l, c, f0, f1;
+  template <bool kLog>
+  __device__ __forceinline__ float at(float x) const {
+    const float d = fmaf(x - m, c, -l);
+    const float p = exp2_(d);
+    return kLog ? p * fmaf(f1, fmaxf(d, kFloor), f0) : p * f0;
+  }
+  // A factor that is not finite must not reach the excluded actions.
+  __device__ __forceinline__ bool odd() const {
+    return !(fabsf(f0) < __builtin_huge_valf()) || !(fabsf(f1) < __builtin_huge_valf()) || l != l;
+  }
+};
+
+// ---- rows of more than kTinyMax actions ----
+
+template <int kOp>
+using ArgsOf = std::conditional_t<kOp == kLogprobs || kOp == kLogprobsTop, LogprobArgs,
+                                  std::conditional_t<kOp == kLogprobsGrad, LogprobGradArgs, DistillArgs>>;
+
+// One workgroup of `nw` waves a row (or a part of one), kN chunks of 16 bytes a
+// lane.  kN = kFewChunks serves short rows, and few rows with more waves each;
+// the longest rows take 16 (8 with a mask, whose bytes want registers too).
+template <class T, bool kMask, int kN, int kOp>
+__global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsOf<kOp> g) {
+  constexpr int kE = kPer<T>;
+  constexpr bool kSums = kOp != kLogprobsGrad && kOp != kDistillGrad;
+  constexpr bool kGrad = kOp == kLogprobsGrad || kOp == kDistillGrad || kOp == kDistillFused;
+  constexpr bool kTop = kOp == kLogprobsTop;
+  constexpr bool kEnt = kOp == kLogprobs || kOp == kLogprobsTop;
+  constexpr bool kTarget = kOp == kDistill || kOp == kDistillFused || kOp == kDistillGrad;
+  constexpr bool kSecond = kTop || kGrad;            // a second pass over the registers
+  constexpr int kHeld = kN == kFewChunks ? 8 : 1;    // target entries a lane keeps
+  using Word = std::conditional_t<kE == 8, uint64_t, uint32_t>;  // a chunk's mask bytes
+  extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
+  __shared__ float red[2][kMaxWaves][8];
+  __shared__ float red2[2][kMaxWaves][2];
+  __shared__ int twice[2];
+  __shared__ std::conditional_t<kTop, TopLds, int> top_lds;
+
+  const int bd = blockDim.x, tid = threadIdx.x;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = bd >> 6;
+  const int lo = blockIdx.y * pt.part;
+  const int len = min(pt.part, a.v - lo);
+  const T* const xb = static_cast<const T*>(a.x) + lo;
+  const uint8_t* const lb = kMask ? a.legal + lo : nullptr;
+
+  u32x4 raw[kN];
+  Word mk[kMask ? kN : 1];
+  // Chunk t of a lane starts at (t * bd + tid) * kE.  Loads never branch: past
+  // `last` (the last whole chunk's start) they repeat that chunk, and what lies
+  // before a chunk's own start is dropped when it is used.
+  int me = tid;  // (renewed for each pass)
+  auto load = [&](int t, const T* x, const uint8_t* legal, int last) {
+    const int oc = min((t * bd + me) * kE, last);
+    raw[t] = load_at<T, u32x4>(x + oc);
+    if constexpr (kMask) mk[t] = load_at<uint8_t, Word>(legal + oc);
+  };
+  // The chunk's values, excluded ones -inf; true where it holds any.
+  auto values = [&](int t, float (&x)[kE]) {
+    unpack<T>(raw[t], x);
+    if constexpr (kMask) {
+#pragma unroll
+      for (int j = 0; j < kE; ++j)
+        if (((mk[t] >> (8 * j)) & 0xFF) == 0) x[j] = neg_inf();
+    }
+    if ((t + 1) * bd * kE > len) {
+      const int o = (t * bd + me) * kE, oc = min(o, len - kE);
+#pragma unroll
+      for (int j = 0; j < kE; ++j)
+        if (oc + j < o) x[j] = neg_inf();
+      if constexpr (kSums && kSecond && !kMask) raw[t] = pack<T>(x);
+    }
+    if constexpr (kSums && kSecond && kMask) raw[t] = pack<T>(x);
+  };
+  // The same again, once values() has left the exclusions in the registers.
+  auto again = [&](int t, float (&x)[kE]) {
+    renew(raw[t]);
+    if constexpr (kSums) unpack<T>(raw[t], x);
+    else values(t, x);
+  };
+
+  int64_t r = blockIdx.x;
+  {
+    const T* x = xb + r * a.ld;
+    const uint8_t* legal = kMask ? lb + r * a.lld : nullptr;
+#pragma unroll
+    for (int t = 0; t < kN; ++t) load(t, x, legal, len - kE);
+  }
+  if constexpr (kTop) {
+    if (tid < 64) top_lds.group[tid] = 0;
+    __syncthreads();
+  }
+
+  for (int par = 0; r < a.n; r += gridDim.x, par ^= 1) {
+    // The next row, loaded as this one's registers come free (after the last
+    // row: one chunk, again and again).
+    const bool more = r + gridDim.x < a.n;
+    const int64_t rn = more ? r + gridDim.x : r;
+    const T* const nx = xb + rn * a.ld;
+    const uint8_t* const nl = kMask ? lb + rn * a.lld : nullptr;
+    const int nlast = more ? len - kE : 0;
+
+    // -- listed entries: load, and their mass --
+    int eid[kTarget ? kHeld : 1];
+    float ez[kTarget ? kHeld : 1], ex[kTarget ? kHeld : 1];
+    Mass mass{neg_inf(), 0.0f};
+    float bad = 0.0f;
+    Table tab{};
+    float* dq = nullptr;
+    bool in_order = false;  // dense LDS: an action listed twice
+    if constexpr (kTarget) {
+      const int k = g.t.k;
+      const auto take = [&](Entry e) {
+        if (e.id >= a.v) bad = 1.0f;
+        mass_add(g.t, a.c, e.z, mass);
+      };
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        eid[i] = -1;
+        ez[i] = neg_inf();
+        ex[i] = neg_inf();
+        if (i * bd < k) {
+          const int j = tid + i * bd;
+          if (j < k) {
+            const Entry e = target_entry(g.t, r, j);
+            take(e);
+            eid[i] = e.id < 0 || e.id >= a.v ? -1 : static_cast<int>(e.id);
+            ez[i] = e.z;
+          }
+        }
+      }
+      for (int j = tid + kHeld * bd; j < k; j += bd) take(target_entry(g.t, r, j));
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        if (i * bd < k && eid[i] >= 0) ex[i] = logit<T>(a, r, eid[i]);
+      if constexpr (kGrad) {
+        if (kN == kFewChunks && nw == 1) {
+          // One wave: the row's weights as an array in LDS.  Each entry leaves
+          // its number; one that finds another's shares its action.
+          dq = reinterpret_cast<float*>(dyn);
+          int* const tag = reinterpret_cast<int*>(dyn);
+          if (g.t.ids != nullptr) {
+            const auto each = [&](auto f) {
+#pragma unroll
+              for (int i = 0; i < kHeld; ++i)
+                if (i * 64 < k && eid[i] >= 0) f(eid[i], tid + i * 64);
+              for (int j = tid + kHeld * 64; j < k; j += 64) {
+                const int64_t id = get_id(g.t.ids, g.t.wide, r * g.t.ids_ld + j);
+                if (id >= 0 && id < a.v) f(static_cast<int>(id), j);
+              }
+            };
+            each([&](int id, int j) { tag[id] = j; });
+            __syncthreads();
+            int clash = 0;
+            each([&](int id, int j) { clash |= tag[id] != j; });
+            in_order = __ballot(clash) != 0;
+            __syncthreads();
+          }
+          for (int i = tid; i < a.v; i += 64) dq[i] = 0.0f;
+          __syncthreads();
+        } else {
+          unsigned char* const base = dyn + static_cast<size_t>(par) * g.hash * 12;
+          tab.key = reinterpret_cast<int32_t*>(base);
+          tab.w = reinterpret_cast<float*>(base + static_cast<size_t>(g.hash) * 4);
+          tab.x = reinterpret_cast<float*>(base + static_cast<size_t>(g.hash) * 8);
+          tab.mask = g.hash - 1;
+          table_clear(tab, tid, bd);
+          if (tid == 0) twice[par] = 0;
+        }
+      }
+    }
+
+    // -- the sums --
+    Sums u{kLowest, 0.0f, 0.0f};
+    int best_o = 0;  // start of the first chunk with the lane's maximum
+    if constexpr (kSums) {
+      renew(me);
+#pragma unroll
+      for (int t = 0; t < kN; ++t) {
+        if (t * bd * kE < len) {
+          float x[kE];
+          values(t, x);
+          float cm = x[0];
+#pragma unroll
+          for (int j = 1; j < kE; ++j) cm = fmaxf(cm, x[j]);
+          if constexpr (kTop) best_o = cm > u.m ? (t * bd + me) * kE : best_o;
+          const float m = fmaxf(u.m, cm);
+          const float dm = (u.m - m) * a.c;
+          const float f = exp2_(dm);
+          if constexpr (kEnt) u.t = f * fmaf(u.s, fmaxf(dm, kFloor), u.t);
+          u.m = m;
+          float s = 0.0f;
+#pragma unroll
+          for (int j = 0; j < kE; ++j) {
+            const float d = (x[j] - m) * a.c;
+            const float e = exp2_(d);
+            s += e;
+            if constexpr (kEnt) u.t = fmaf(e, fmaxf(d, kFloor), u.t);
+          }
+          u.s = fmaf(u.s, f, s);
+        }
+        if constexpr (!kSecond) load(t, nx, nl, nlast);
+      }
+    }
+
+    // -- across the lanes and waves --
+    uint64_t lane_key = 0;
+    if constexpr (kTop) {
+      if (u.s > 0.0f) lane_key = top_key(u.m, static_cast<uint32_t>(lo + best_o));
+      if (nw > 1 && lane_key != 0)
+        atomicMax(reinterpret_cast<unsigned long long*>(&top_lds.group[lane]),
+                  static_cast<unsigned long long>(lane_key));
+    }
+    if constexpr (kSums) u = fold_sums<kEnt>(u, a.c);
+    if constexpr (kTarget) {
+      mass = mass_fold(g.t, a.c, mass, [](float z) { return fold64(z, Max{}); },
+                       [](float z) { return fold64(z, Add{}); });
+      bad = fold64(bad, Max{});
+    }
+    if (nw > 1) {
+      if (lane == 0) {
+        float* const q = red[par][wave];
+        q[0] = u.m;
+        q[1] = u.s;
+        q[2] = u.t;
+        q[3] = mass.z;
+        q[4] = mass.s;
+        q[5] = bad;
+      }
+      __syncthreads();
+      const float* const q = red[par][lane & (kMaxWaves - 1)];
+      const bool in = lane < nw;
+      if constexpr (kSums) {
+        u = in ? Sums{q[0], q[1], q[2]} : Sums{kLowest, 0.0f, 0.0f};
+        u = fold_sums<kEnt>(u, a.c);
+      }
+      if constexpr (kTarget) {
+        mass = in ? Mass{q[3], q[4]} : Mass{neg_inf(), 0.0f};
+        mass = mass_fold(g.t, a.c, mass, [](float z) { return fold64(z, Max{}); },
+                         [](float z) { return fold64(z, Add{}); });
+        bad = fold64(in ? q[5] : 0.0f, Max{});
+      }
+    }
+    float m, l;
+    if constexpr (kSums) {
+      m = u.s == 0.0f ? 0.0f : u.m;
+      l = u.s == 0.0f ? 0.0f : log2f(u.s);
+    } else {
+      m = g.stats[2 * r];
+      l = g.stats[2 * r + 1];
+    }
+
+    // -- log probabilities --
+    if constexpr (kOp == kLogprobs || kOp == kLogprobsTop) {
+      const int64_t part = r * pt.parts + blockIdx.y;
+      if (tid == 0) {
+        if (g.sums != nullptr) {
+          g.sums[part] = PartSums{u.m, u.s, u.t, 0.0f};
+        } else {
+          g.entropy[r] = kLn2 * (l - (u.s == 0.0f ? 0.0f : u.t / u.s));
+          if (g.stats != nullptr) {
+            g.stats[2 * r] = m;
+            g.stats[2 * r + 1] = l;
+          }
+          if (g.actions != nullptr) {
+            const int64_t id = get_id(g.actions, g.wide, r);
+            g.logprob[r] = id < 0 ? 0.0f
+                           : id >= a.v ? __builtin_nanf("")
+                                       : log_p(a, logit<T>(a, r, id), m, l);
+          }
+        }
+      }
+      if constexpr (kTop) {
+        // The top-th largest of 64 lane maxima bounds the row's top-th largest
+        // from below; ties are cut at the end of the chunk that holds it, so
+        // what passes is a beginning of the order (value, then index) and has
+        // `top` entries or all there are.  Usually a few more: they are ranked
+        // by counting.  (The lanes' maxima are known from the sums; a selection
+        // without the bound costs a pass over the row for each of `top`.)
+        if (wave == 0) {
+          const uint64_t key = nw == 1 ? lane_key : top_lds.group[lane];
+          const uint64_t lim = kth64(key, g.top);
+          top_lds.group[lane] = 0;
+          if (lane == 0) {
+            top_lds.limit = lim;
+            top_lds.count = 0;
+          }
+        }
+        __syncthreads();
+        const uint64_t lim = top_lds.limit;
+        const bool odd = l != l;
+        const float tv = lim == 0 ? neg_inf() : key_value(lim);
+        const int ti = lim == 0 ? 0 : static_cast<int>(key_index(lim)) - lo + kE;
+        renew(me);
+#pragma unroll
+        for (int t = 0; t < kN; ++t) {
+          if (t * bd * kE < len && !odd) {
+            float x[kE];
+            again(t, x);
+            float cm = x[0];
+#pragma unroll
+            for (int j = 1; j < kE; ++j) cm = fmaxf(cm, x[j]);
+            const int o = (t * bd + me) * kE;
+            if (cm > tv || (cm == tv && o < ti)) {
+              const int oc = min(o, len - kE);
+#pragma unroll
+              for (int j = 0; j < kE; ++j)
+                if (x[j] > tv || (x[j] == tv && oc + j < ti)) {
+                  const uint32_t at = atomicAdd(&top_lds.count, 1u);
+                  if (at < kCandidates)
+                    top_lds.cand[at] = top_key(x[j], static_cast<uint32_t>(lo + oc + j));
+                }
+            }
+          }
+          load(t, nx, nl, nlast);
+        }
+        __syncthreads();
+        const int found = odd ? 0 : static_cast<int>(top_lds.count);
+        const auto put = [&](int rank, uint64_t key) {
+          if (g.part_keys != nullptr) {
+            g.part_keys[part * g.top + rank] = key;
+            return;
+          }
+          g.top_action[r * g.top + rank] = key == 0 ? -1 : static_cast<int64_t>(key_index(key));
+          g.top_logprob[r * g.top + rank] =
+              odd ? l : key == 0 ? neg_inf() : log_p(a, key_value(key), m, l);
+        };
+        if (found <= kCandidates) {
+          for (int i = tid; i < found; i += bd) {
+            const uint64_t key = top_lds.cand[i];
+            int rank = 0;
+            for (int j = 0; j < found; ++j) rank += top_lds.cand[j] > key ? 1 : 0;
+            if (rank < g.top) put(rank, key);
+          }
+          for (int i = found + tid; i < g.top; i += bd) put(i, 0);
+        } else {
+          // Hundreds of the largest values in fewer lanes than `top`: one
+          // round over the row for each, from memory.
+          uint64_t last = ~0ull;
+          for (int k = 0; k < g.top; ++k) {
+            uint64_t best = 0;
+            for (int i = tid; i < len; i += bd) {
+              const float x = logit<T>(a, r, lo + i);
+              const uint64_t key = top_key(x, static_cast<uint32_t>(lo + i));
+              if (x > neg_inf() && key < last && key > best) best = key;
+            }
+            best = fold64_max(best);
+            __syncthreads();
+            if (lane == 0) top_lds.cand[wave] = best;
+            __syncthreads();
+            for (int w = 0; w < nw; ++w) best = top_lds.cand[w] > best ? top_lds.cand[w] : best;
+            if (tid == 0) put(k, best);
+            last = best;
+          }
+        }
+      }
+    }
+
+    // -- distillation: loss, and the listed weights --
+    float f0 = 0.0f, f1 = 0.0f, scale = 0.0f, inv = 0.0f;
+    if constexpr (kTarget) {
+      inv = mass.s == 0.0f ? 0.0f : 1.0f / mass.s;
+      if constexpr (kGrad) {
+        scale = (g.weight != nullptr ? g.weight[r * g.weight_stride] : 1.0f) * a.inv_t;
+        f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
+      }
+      float ce = 0.0f, h = 0.0f;
+      const auto use = [&](int id, float z, float x) {
+        const float q = target_mass(g.t, a.c, z, mass.z) * inv;
+        if constexpr (kOp != kDistillGrad) {
+          if (q != 0.0f) {
+            if (id >= 0) ce -= q * log_p(a, x, m, l);
+            h -= q * (kLn2 * log2f(q));
+          }
+        }
+        if constexpr (kGrad) {
+          if (id >= 0 && x > neg_inf()) {
+            if (dq != nullptr) {
+              if (!in_order) dq[id] = -scale * q;
+            } else if (id >= lo && id < lo + len) {
+              if (!table_put(tab, id, -scale * q, x)) twice[par] = 1;
+            }
+          }
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        if (i * bd < g.t.k) use(eid[i], ez[i], ex[i]);
+      for (int j = tid + kHeld * bd; j < g.t.k; j += bd) {
+        const Entry e = target_entry(g.t, r, j);
+        const int id = e.id < 0 || e.id >= a.v ? -1 : static_cast<int>(e.id);
+        use(id, e.z, id < 0 ? neg_inf() : logit<T>(a, r, id));
+      }
+      if constexpr (kGrad) {
+        if (dq != nullptr) {
+          __syncthreads();
+          if (in_order) {
+            if (tid == 0)
+              for (int j = 0; j < g.t.k; ++j) {
+                const Entry e = target_entry(g.t, r, j);
+                if (e.id >= 0 && e.id < a.v && logit<T>(a, r, e.id) > neg_inf())
+                  dq[e.id] -= scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
+              }
+            __syncthreads();
+          }
+        }
+      }
+      if constexpr (kOp != kDistillGrad) {
+        ce = fold64(ce, Add{});
+        h = fold64(h, Add{});
+        const auto out = [&] {
+          g.loss[r] = bad != 0.0f ? __builtin_nanf("") : ce;
+          if (g.tent != nullptr) g.tent[r] = h;
+          if (g.stats != nullptr) {
+            g.stats[2 * r] = m;
+            g.stats[2 * r + 1] = l;
+          }
+        };
+        if (nw == 1) {
+          if (tid == 0) out();
+        } else {
+          if (lane == 0) {
+            red2[par][wave][0] = ce;
+            red2[par][wave][1] = h;
+          }
+          __syncthreads();
+          if (tid == 0) {
+            for (int w = 1; w < nw; ++w) {
+              ce += red2[par][w][0];
+              h += red2[par][w][1];
+            }
+            out();
+          }
+        }
+      }
+    }
+
+    // -- gradient of the log probabilities: factors and listed weights --
+    int act = -1;
+    float act_w = 0.0f, act_x = neg_inf();
+    if constexpr (kOp == kLogprobsGrad) {
+      const int64_t id = g.actions != nullptr && g.gl != nullptr ? get_id(g.actions, g.wide, r) : -1;
+      float sum = id >= a.v ? __builtin_nanf("") : 0.0f;
+      if (id >= 0 && id < a.v) {
+        act = static_cast<int>(id);
+        act_w = g.gl[r * g.gls];
+        sum = act_w;
+        act_w *= a.inv_t;
+        act_x = logit<T>(a, r, id);
+      }
+      if (g.top > 0) {
+        int64_t ti = -1;
+        float gt = 0.0f;
+        if (lane < g.top) {
+          ti = g.top_action[r * g.top + lane];
+          gt = ti >= 0 && ti < a.v ? g.gt[r * g.top + lane] : 0.0f;
+        }
+        sum += fold64(gt, Add{});
+        unsigned char* const base = dyn + static_cast<size_t>(par) * 128 * 12;
+        tab.key = reinterpret_cast<int32_t*>(base);
+        tab.w = reinterpret_cast<float*>(base + 128 * 4);
+        tab.x = reinterpret_cast<float*>(base + 128 * 8);
+        tab.mask = 127;
+        table_clear(tab, tid, bd);
+        if (tid == 0) twice[par] = 0;
+        __syncthreads();
+        if (wave == 0 && ti >= lo && ti < lo + len) {
+          const float x = logit<T>(a, r, ti);
+          if (x > neg_inf() && !table_put(tab, static_cast<int>(ti), gt * a.inv_t, x)) twice[par] = 1;
+        }
+      }
+      const float gh = g.gh != nullptr ? g.gh[r * g.ghs] : 0.0f;
+      f0 = -(sum + (gh != 0.0f ? gh * g.entropy[r] : 0.0f)) * a.inv_t;
+      f1 = -gh * kLn2 * a.inv_t;
+    }
+
+    // -- the gradient --
+    if constexpr (kGrad) {
+      const Dense dn{m, l, a.c, f0, f1};
+      constexpr bool kLog = kOp == kLogprobsGrad;
+      const bool odd = dn.odd();
+      T* const gb = static_cast<T*>(g.grad) + r * g.grad_ld + lo;
+      renew(me);
+#pragma unroll
+      for (int t = 0; t < kN; ++t) {
+        if (t * bd * kE < len) {
+          float x[kE], y[kE];
+          again(t, x);
+          const int o = (t * bd + me) * kE, oc = min(o, len - kE);
+#pragma unroll
+          for (int j = 0; j < kE; ++j) y[j] = dn.template at<kLog>(x[j]);
+          if (odd) {
+#pragma unroll
+            for (int j = 0; j < kE; ++j) y[j] = x[j] == neg_inf() ? 0.0f : y[j];
+          }
+          if constexpr (kTarget && kN == kFewChunks) {
+            if (dq != nullptr) {
+#pragma unroll
+              for (int j = 0; j < kE; ++j) y[j] += dq[oc + j];
+            }
+          }
+          if (o + kE <= len) {
+            store_at<T>(gb + o, pack<T>(y));
+          } else if (o < len) {
+#pragma unroll
+            for (int j = 0; j < kE; ++j)
+              if (oc + j >= o) gb[oc + j] = static_cast<T>(y[j]);
+          }
+        }
+        load(t, nx, nl, nlast);
+      }
+      // the listed actions once more, with their weights (a barrier: after the
+      // dense stores of whichever wave)
+      const auto fix = [&](int id, float w, float x) {
+        gb[id - lo] = static_cast<T>(dn.template at<kLog>(x) + w);
+      };
+      if constexpr (kTarget) {
+        if (dq == nullptr) {
+          __syncthreads();
+          if (twice[par] != 0) {
+            __syncthreads();
+            table_clear(tab, tid, bd);
+            __syncthreads();
+            if (tid == 0)
+              for (int j = 0; j < g.t.k; ++j) {
+                const Entry e = target_entry(g.t, r, j);
+                if (e.id < lo || e.id >= lo + len) continue;
+                const float x = logit<T>(a, r, e.id);
+                if (x > neg_inf())
+                  table_add(tab, static_cast<int>(e.id),
+                            -scale * (target_mass(g.t, a.c, e.z, mass.z) * inv), x);
+              }
+            __syncthreads();
+          }
+          for (int i = tid; i <= tab.mask; i += bd)
+            if (tab.key[i] >= 0) fix(tab.key[i], tab.w[i], tab.x[i]);
+        } else {
+          __syncthreads();  // dq is the next row's
+        }
+      } else {
+        __syncthreads();
+        const bool mine = act >= lo && act < lo + len && act_x > neg_inf();
+        if (g.top == 0) {
+          if (tid == 0 && mine) fix(act, act_w, act_x);
+        } else {
+          const bool again_ = twice[par] != 0;
+          if (again_) {
+            __syncthreads();
+            table_clear(tab, tid, bd);
+            __syncthreads();
+          }
+          if (tid == 0) {
+            if (again_)
+              for (int j = 0; j < g.top; ++j) {
+                const int64_t id = g.top_action[r * g.top + j];
+                if (id < lo || id >= lo + len) continue;
+                const float x = logit<T>(a, r, id);
+                if (x > neg_inf())
+                  table_add(tab, static_cast<int>(id), g.gt[r * g.top + j] * a.inv_t, x);
+              }
+            if (mine) table_add(tab, act, act_w, act_x);
+          }
+          __syncthreads();
+          for (int i = tid; i <= tab.mask; i += bd)
+            if (tab.key[i] >= 0) fix(tab.key[i], tab.w[i], tab.x[i]);
+        }
+      }
+    }
+  }
+}
+
+// ---- joining a row's parts ----
+
+// One workgroup of kJoin lanes a row: the parts' sums (a lane each), then their
+// top lists or the loss.
+constexpr int kJoin = 256;
+
+template <class T, bool kLoss>
+__global__ __launch_bounds__(kJoin) void k_join(Rows a, JoinArgs g) {
+  __shared__ uint64_t cand[kLoss ? 1 : kMaxSplit * OS_AZ_MAX_TOP];
+  __shared__ uint32_t count;
+  __shared__ float red[kJoin / 64][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r = blockIdx.x;
+  const PartSums* const ps = g.lp.sums + r * g.parts;
+  Sums u{kLowest, 0.0f, 0.0f};
+  if (lane < g.parts) u = Sums{ps[lane].m, ps[lane].s, ps[lane].t};
+  u = fold_sums<!kLoss>(u, a.c);
+  const float m = u.s == 0.0f ? 0.0f : u.m;
+  const float l = u.s == 0.0f ? 0.0f : log2f(u.s);
+  float* const stats = kLoss ? g.ds.stats : g.lp.stats;
+  if (tid == 0 && stats != nullptr) {
+    stats[2 * r] = m;
+    stats[2 * r + 1] = l;
+  }
+  if constexpr (!kLoss) {
+    const LogprobArgs& q = g.lp;
+    if (tid == 0) {
+      q.entropy[r] = kLn2 * (l - (u.s == 0.0f ? 0.0f : u.t / u.s));
+      if (q.actions != nullptr) {
+        const int64_t id = get_id(q.actions, q.wide, r);
+        q.logprob[r] = id < 0 ? 0.0f
+                       : id >= a.v ? __builtin_nanf("")
+                                   : log_p(a, logit<T>(a, r, id), m, l);
+      }
+      count = 0;
+    }
+    if (q.top == 0) return;
+    // Each list is in order.  With `deep` = ceil(top / parts) entries a list,
+    // the ceil(top / deep)-th largest of the lists' deep-th entries has at
+    // least `top` entries at or above it.
+    const int deep = (q.top + g.parts - 1) / g.parts;
+    const int need = (q.top + deep - 1) / deep;
+    const uint64_t* const keys = q.part_keys + r * g.parts * q.top;
+    const uint64_t lim = kth64(lane < g.parts ? keys[lane * q.top + deep - 1] : 0, need);
+    __syncthreads();
+    const bool odd = l != l;
+    if (!odd)
+      for (int i = tid; i < g.parts * q.top; i += kJoin) {
+        const uint64_t k = keys[i];
+        if (k != 0 && k >= lim) cand[atomicAdd(&count, 1u)] = k;
+      }
+    __syncthreads();
+    const int found = static_cast<int>(count);
+    const auto put = [&](int rank, uint64_t key) {
+      q.top_action[r * q.top + rank] = key == 0 ? -1 : static_cast<int64_t>(key_index(key));
+      q.top_logprob[r * q.top + rank] =
+          odd ? l : key == 0 ? neg_inf() : log_p(a, key_value(key), m, l);
+    };
+    for (int i = tid; i < found; i += kJoin) {
+      const uint64_t key = cand[i];
+      int rank = 0;
+      for (int j = 0; j < found; ++j) rank += cand[j] > key ? 1 : 0;
+      if (rank < q.top) put(rank, key);
+    }
+    for (int i = found + tid; i < q.top; i += kJoin) put(i, 0);
+  } else {
+    const DistillArgs& q = g.ds;
+    Mass mass{neg_inf(), 0.0f};
+    float bad = 0.0f;
+    for (int j = tid; j < q.t.k; j += kJoin) {
+      const Entry e = target_entry(q.t, r, j);
+      if (e.id >= a.v) bad = 1.0f;
+      mass_add(q.t, a.c, e.z, mass);
+    }
+    const auto maxf = [](float z) { return fold64(z, Max{}); };
+    const auto addf = [](float z) { return fold64(z, Add{}); };
+    mass = mass_fold(q.t, a.c, mass, maxf, addf);
+    bad = fold64(bad, Max{});
+    if (lane == 0) {
+      red[wave][0] = mass.z;
+      red[wave][1] = mass.s;
+      red[wave][2] = bad;
+    }
+    __syncthreads();
+    const bool in = lane < kJoin / 64;
+    const float* const w0 = red[lane & (kJoin / 64 - 1)];
+    mass = in ? Mass{w0[0], w0[1]} : Mass{neg_inf(), 0.0f};
+    bad = fold64(in ? w0[2] : 0.0f, Max{});
+    mass = mass_fold(q.t, a.c, mass, maxf, addf);
+    const float inv = mass.s == 0.0f ? 0.0f : 1.0f / mass.s;
+    float ce = 0.0f, h = 0.0f;
+    for (int j = tid; j < q.t.k; j += kJoin) {
+      const Entry e = target_entry(q.t, r, j);
+      const float p = target_mass(q.t, a.c, e.z, mass.z) * inv;
+      if (p == 0.0f) continue;
+      if (e.id >= 0 && e.id < a.v) ce -= p * log_p(a, logit<T>(a, r, e.id), m, l);
+      h -= p * (kLn2 * log2f(p));
+    }
+    ce = fold64(ce, Add{});
+    h = fold64(h, Add{});
+    __syncthreads();
+    if (lane == 0) {
+      red[wave][0] = ce;
+      red[wave][1] = h;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < kJoin / 64; ++w) {
+        ce += red[w][0];
+        h += red[w][1];
+      }
+      q.loss[r] = bad != 0.0f ? __builtin_nanf("") : ce;
+      if (q.tent != nullptr) q.tent[r] = h;
+    }
+  }
+}
+
+// ---- rows of up to kTinyMax actions ----
+
+// 16 lanes a row (one DPP row: reductions need no LDS), four elements a lane,
+// 16 apart; 16 rows a workgroup.  A wave a row would leave most lanes idle at
+// these sizes, a lane a row would leave the card empty at a few thousand rows.
+constexpr int kTinyBlock = 256;
+constexpr int kTinyRows = kTinyBlock / 16;
+
+template <class T, int kOp>
+__global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
+  constexpr bool kSums = kOp != kLogprobsGrad && kOp != kDistillGrad;
+  constexpr bool kGrad = kOp == kLogprobsGrad || kOp == kDistillGrad || kOp == kDistillFused;
+  constexpr bool kTarget = kOp == kDistill || kOp == kDistillFused || kOp == kDistillGrad;
+  constexpr int kEach = kTinyMax / 16;
+  __shared__ float lds[kGrad ? kTinyRows : 1][kTinyMax];
+  const int tid = threadIdx.x, l16 = tid & 15, sub = tid >> 4;
+  float* const dq = lds[kGrad ? sub : 0];
+  const Max maxf{};
+  const Add addf{};
+  // Whole workgroups go round together (barriers): a row past the end repeats
+  // the last one and writes nothing.
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kTinyRows; r0 < a.n;
+       r0 += static_cast<int64_t>(gridDim.x) * kTinyRows) {
+    const bool live = r0 + sub < a.n;
+    const int64_t r = live ? r0 + sub : a.n - 1;
+    float x[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      x[e] = neg_inf();
+      const int i = l16 + 16 * e;
+      if (16 * e < a.v && i < a.v) x[e] = logit<T>(a, r, i);
+    }
+    float m, l, mean = 0.0f;
+    if constexpr (kSums) {
+      float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      mx = fold16(mx, maxf);
+      m = mx == neg_inf() ? 0.0f : mx;  // empty, or only NaN
+      float s = 0.0f, t = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const float d = (x[e] - m) * a.c;
+        const float p = exp2_(d);
+        s += p;
+        t = fmaf(p, fmaxf(d, kFloor), t);
+      }
+      s = fold16(s, addf);
+      t = fold16(t, addf);
+      l = s == 0.0f ? 0.0f : log2f(s);
+      mean = s == 0.0f ? 0.0f : t / s;
+    } else {
+      m = g.stats[2 * r];
+      l = g.stats[2 * r + 1];
+    }
+    if constexpr (kOp == kLogprobs || kOp == kLogprobsTop) {
+      if (l16 == 0 && live) {
+        g.entropy[r] = kLn2 * (l - mean);
+        if (g.stats != nullptr) {
+          g.stats[2 * r] = m;
+          g.stats[2 * r + 1] = l;
+        }
+        if (g.actions != nullptr) {
+          const int64_t id = get_id(g.actions, g.wide, r);
+          g.logprob[r] = id < 0 ? 0.0f
+                         : id >= a.v ? __builtin_nanf("")
+                                     : log_p(a, logit<T>(a, r, id), m, l);
+        }
+      }
+      if constexpr (kOp == kLogprobsTop) {
+        const bool odd = l != l;
+        for (int k = 0; k < g.top; ++k) {
+          float best = odd ? neg_inf() : fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          best = fold16(best, maxf);
+          uint32_t at = 0xFFFFFFFFu;
+#pragma unroll
+          for (int e = kEach - 1; e >= 0; --e)
+            if (x[e] == best && best > neg_inf()) at = static_cast<uint32_t>(l16 + 16 * e);
+          at = fold16(at, MinU{});
+#pragma unroll
+          for (int e = 0; e < kEach; ++e)
+            if (static_cast<uint32_t>(l16 + 16 * e) == at) x[e] = neg_inf();
+          if (l16 == 0 && live) {
+            const bool none = best == neg_inf();
+            g.top_action[r * g.top + k] = none ? -1 : static_cast<int64_t>(at);
+            g.top_logprob[r * g.top + k] = odd ? l : none ? best : log_p(a, best, m, l);
+          }
+        }
+      }
+    }
+    Dense dn{m, l, a.c, 0.0f, 0.0f};
+    if constexpr (kGrad) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) dq[l16 + 16 * e] = 0.0f;
+      __syncthreads();
+    }
+    if constexpr (kTarget) {
+      Mass mass{neg_inf(), 0.0f};
+      float bad = 0.0f;
+      int* const tag = reinterpret_cast<int*>(dq);
+      for (int j = l16; j < g.t.k; j += 16) {
+        const Entry e = target_entry(g.t, r, j);
+        if (e.id >= a.v) bad = 1.0f;
+        else if (kGrad && e.id >= 0) tag[e.id] = j;
+        mass_add(g.t, a.c, e.z, mass);
+      }
+      mass = mass_fold(g.t, a.c, mass, [&](float z) { return fold16(z, maxf); },
+                       [&](float z) { return fold16(z, addf); });
+      bad = fold16(bad, maxf);
+      const float inv = mass.s == 0.0f ? 0.0f : 1.0f / mass.s;
+      float scale = 0.0f;
+      if constexpr (kGrad)
+        scale = (g.weight != nullptr ? g.weight[r * g.weight_stride] : 1.0f) * a.inv_t;
+      float clash = 0.0f;
+      if constexpr (kGrad) {
+        // an entry that finds another's number shares its action
+        __syncthreads();
+        for (int j = l16; j < g.t.k; j += 16) {
+          const int64_t id = g.t.ids != nullptr ? get_id(g.t.ids, g.t.wide, r * g.t.ids_ld + j) : j;
+          if (id >= 0 && id < a.v && tag[id] != j) clash = 1.0f;
+        }
+        clash = fold16(clash, maxf);
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) dq[l16 + 16 * e] = 0.0f;
+        __syncthreads();
+      }
+      float ce = 0.0f, h = 0.0f;
+      for (int j = l16; j < g.t.k; j += 16) {
+        const Entry e = target_entry(g.t, r, j);
+        const float q = target_mass(g.t, a.c, e.z, mass.z) * inv;
+        const bool in = e.id >= 0 && e.id < a.v;
+        if constexpr (kOp != kDistillGrad) {
+          if (q != 0.0f) {
+            if (in) ce -= q * log_p(a, logit<T>(a, r, e.id), m, l);
+            h -= q * (kLn2 * log2f(q));
+          }
+        }
+        if (kGrad && in && clash == 0.0f) dq[e.id] = -scale * q;
+      }
+      if constexpr (kOp != kDistillGrad) {
+        ce = fold16(ce, addf);
+        h = fold16(h, addf);
+        if (l16 == 0 && live) {
+          g.loss[r] = bad != 0.0f ? __builtin_nanf("") : ce;
+          if (g.tent != nullptr) g.tent[r] = h;
+          if (g.stats != nullptr) {
+            g.stats[2 * r] = m;
+            g.stats[2 * r + 1] = l;
+          }
+        }
+      }
+      if constexpr (kGrad) {
+        if (clash != 0.0f && l16 == 0)
+          for (int j = 0; j < g.t.k; ++j) {
+            const Entry e = target_entry(g.t, r, j);
+            if (e.id >= 0 && e.id < a.v)
+              dq[e.id] -= scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
+          }
+        dn.f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
+        __syncthreads();
+      }
+    }
+    if constexpr (kOp == kLogprobsGrad) {
+      const int64_t id = g.actions != nullptr && g.gl != nullptr ? get_id(g.actions, g.wide, r) : -1;
+      float sum = id >= a.v ? __builtin_nanf("") : 0.0f;
+      const float gl = id >= 0 && id < a.v ? g.gl[r * g.gls] : 0.0f;
+      sum += gl;
+      if (l16 == 0) {  // (in list order: an action may be met twice)
+        for (int j = 0; j < g.top; ++j) {
+          const int64_t ti = g.top_action[r * g.top + j];
+          if (ti < 0 || ti >= a.v) continue;
+          const float w = g.gt[r * g.top + j];
+          sum += w;
+          dq[ti] += w * a.inv_t;
+        }
+        if (id >= 0 && id < a.v) dq[id] += gl * a.inv_t;
+      }
+      sum = __shfl(sum, tid & 48);  // the row's first lane's
+      const float gh = g.gh != nullptr ? g.gh[r * g.ghs] : 0.0f;
+      dn.f0 = -(sum + (gh != 0.0f ? gh * g.entropy[r] : 0.0f)) * a.inv_t;
+      dn.f1 = -gh * kLn2 * a.inv_t;
+      __syncthreads();
+    }
+    if constexpr (kGrad) {
+      T* const gb = static_cast<T*>(g.grad) + r * g.grad_ld;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int i = l16 + 16 * e;
+        if (i < a.v && live) {
+          const float y = dn.template at<kOp == kLogprobsGrad>(x[e]) + dq[i];
+          gb[i] = static_cast<T>(x[e] == neg_inf() ? 0.0f : y);
+        }
+      }
+      __syncthreads();  // dq is the next rows'
+    }
+  }
+}
+
+// ---- launches (one unit a type) ----
+
+struct Launch {
+  Rows a;
+  Parts pt;
+  dim3 grid;
+  int waves;       // 0: k_tiny
+  bool few;        // kFewChunks chunks a lane
+  unsigned lds;    // dynamic, bytes
+  hipStream_t stream;
+};
+
+template <class T>
+struct Kernels {
+  static void rows(const Launch& c, int op, const LogprobArgs& g);
+  static void rows(const Launch& c, const LogprobGradArgs& g);
+  static void rows(const Launch& c, int op, const DistillArgs& g);
+  static void join(const Launch& c, bool loss, const JoinArgs& g);
+};
+
+}  // namespace osp
+
+#endif  // OS_POLICY_H_

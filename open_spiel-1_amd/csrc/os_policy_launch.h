@@ -1,0 +1,52 @@
+// Instantiates the policy kernels (os_policy.h) for one element type.
+#ifndef OS_POLICY_LAUNCH_H_
+#define OS_POLICY_LAUNCH_H_
+
+#include "os_policy.h"
+
+namespace osp {
+
+template <class T, int kOp, class G>
+void launch_rows(const Launch& c, const G& g) {
+  if (c.waves == 0) {
+    hipLaunchKernelGGL((k_tiny<T, kOp>), c.grid, dim3(kTinyBlock), 0, c.stream, c.a, g);
+    return;
+  }
+  const dim3 block(64 * c.waves);
+  if (c.a.legal != nullptr) {
+    if (c.few)
+      hipLaunchKernelGGL((k_rows<T, true, kFewChunks, kOp>), c.grid, block, c.lds, c.stream, c.a, c.pt, g);
+    else
+      hipLaunchKernelGGL((k_rows<T, true, kMaskChunks, kOp>), c.grid, block, c.lds, c.stream, c.a, c.pt, g);
+  } else {
+    if (c.few)
+      hipLaunchKernelGGL((k_rows<T, false, kFewChunks, kOp>), c.grid, block, c.lds, c.stream, c.a, c.pt, g);
+    else
+      hipLaunchKernelGGL((k_rows<T, false, kChunks, kOp>), c.grid, block, c.lds, c.stream, c.a, c.pt, g);
+  }
+}
+
+template <class T>
+void Kernels<T>::rows(const Launch& c, int op, const LogprobArgs& g) {
+  if (op == kLogprobs) launch_rows<T, kLogprobs>(c, g);
+  else launch_rows<T, kLogprobsTop>(c, g);
+}
+template <class T>
+void Kernels<T>::rows(const Launch& c, const LogprobGradArgs& g) {
+  launch_rows<T, kLogprobsGrad>(c, g);
+}
+template <class T>
+void Kernels<T>::rows(const Launch& c, int op, const DistillArgs& g) {
+  if (op == kDistill) launch_rows<T, kDistill>(c, g);
+  else if (op == kDistillFused) launch_rows<T, kDistillFused>(c, g);
+  else launch_rows<T, kDistillGrad>(c, g);
+}
+template <class T>
+void Kernels<T>::join(const Launch& c, bool loss, const JoinArgs& g) {
+  if (loss) hipLaunchKernelGGL((k_join<T, true>), c.grid, dim3(kJoin), 0, c.stream, c.a, g);
+  else hipLaunchKernelGGL((k_join<T, false>), c.grid, dim3(kJoin), 0, c.stream, c.a, g);
+}
+
+}  // namespace osp
+
+#endif  // OS_POLICY_LAUNCH_H_

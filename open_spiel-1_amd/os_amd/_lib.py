@@ -214,7 +214,7 @@ _sig("os_az_distill_grad_async", ctypes.c_int,
      [_rows_p, _target_p, _vp, _i64, _vp, _vp, _i64, _vp])
 AZ_F32, AZ_BF16, AZ_F16 = 0, 1, 2
 AZ_LOGITS_F32, AZ_LOGITS_BF16, AZ_LOGITS_F16, AZ_WEIGHTS_F32, AZ_WEIGHTS_I32 = range(5)
-AZ_MAX_ACTIONS, AZ_MAX_TOP, AZ_MAX_TARGETS = 4194304, 64, 1024
+AZ_MAX_ACTIONS, AZ_MAX_TOP, AZ_MAX_TARGETS = 2097152, 64, 1024
 _sig("os_az_fetch", ctypes.c_int, [_vp, _i32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P])
 _sig("os_engine_node_bytes", _i32, [_vp])
 _sig("os_engine_state_bytes", _i32, [_vp])

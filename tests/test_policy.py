@@ -717,7 +717,7 @@ def _c_target(**kw):
 
 
 BAD_ROWS = [dict(logits=None), dict(num_rows=-1), dict(ld=-1), dict(legal_ld=-1),
-            dict(num_actions=0), dict(num_actions=4194305), dict(dtype=-1), dict(dtype=3),
+            dict(num_actions=0), dict(num_actions=2097153), dict(dtype=-1), dict(dtype=3),
             dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=math.inf),
             dict(temperature=math.nan), dict(temperature=1e-38), dict(reserved=1),
             dict(logits=4098), dict(logits=4097, dtype=1)]
