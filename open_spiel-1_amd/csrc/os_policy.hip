@@ -18,6 +18,8 @@ using namespace osp;
 constexpr int kCus = 256;
 constexpr int64_t kKib = 1024;
 constexpr int64_t kWaveFew = kFewChunks * kKib;  // bytes a wave holds: 64 lanes x 16 a chunk
+// (sums_plan leaves rows of up to four such waves whole)
+static_assert(OS_AZ_NO_WORKSPACE_ACTIONS * 4 <= 4 * kWaveFew);
 
 // ---- how the workgroups share the rows ----
 

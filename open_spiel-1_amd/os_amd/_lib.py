@@ -202,7 +202,7 @@ _sig("os_az_prepare_staged", ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp])
 _sig("os_az_set_noise", ctypes.c_int, [_vp, _P, _i64, ctypes.c_double])
 _sig("os_az_tree_priors", ctypes.c_int, [_vp, _i64, _i64, _P])
 AZ_REQUESTS_SEPARATE, AZ_REQUESTS_FUSED = 0, 1
-_rows_p, _target_p = ctypes.POINTER(AzRows), ctypes.POINTER(AzTarget)
+_rows_p, _target_p = _vp, _vp  # (bytes packed as the struct, or byref)
 _sig("os_az_rows_workspace", _i64, [_rows_p, _i32])
 _sig("os_az_logprobs_async", ctypes.c_int,
      [_rows_p, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp])
@@ -215,6 +215,8 @@ _sig("os_az_distill_grad_async", ctypes.c_int,
 AZ_F32, AZ_BF16, AZ_F16 = 0, 1, 2
 AZ_LOGITS_F32, AZ_LOGITS_BF16, AZ_LOGITS_F16, AZ_WEIGHTS_F32, AZ_WEIGHTS_I32 = range(5)
 AZ_MAX_ACTIONS, AZ_MAX_TOP, AZ_MAX_TARGETS = 2097152, 64, 1024
+AZ_NO_WORKSPACE_ACTIONS = 4096
+AZ_ROWS_BYTES, AZ_TARGET_BYTES = ctypes.sizeof(AzRows), ctypes.sizeof(AzTarget)
 _sig("os_az_fetch", ctypes.c_int, [_vp, _i32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P])
 _sig("os_engine_node_bytes", _i32, [_vp])
 _sig("os_engine_state_bytes", _i32, [_vp])

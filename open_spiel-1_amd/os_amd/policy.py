@@ -31,7 +31,7 @@ calls, or with torch.autograd.grad: like any autograd operator, a `.backward()`
 captured while an eager graph of the same leaves is alive is not supported by
 torch.
 """
-import ctypes
+import struct
 from typing import NamedTuple, Optional
 
 import numpy as np
@@ -40,15 +40,28 @@ import torch
 from . import _lib
 from ._lib import check, lib
 
+_F32 = torch.float32
 _DTYPES = {torch.float32: _lib.AZ_F32, torch.bfloat16: _lib.AZ_BF16, torch.float16: _lib.AZ_F16}
 _TARGETS = {
-    ("logits", torch.float32): _lib.AZ_LOGITS_F32,
-    ("logits", torch.bfloat16): _lib.AZ_LOGITS_BF16,
-    ("logits", torch.float16): _lib.AZ_LOGITS_F16,
-    ("weights", torch.float32): _lib.AZ_WEIGHTS_F32,
-    ("weights", torch.int32): _lib.AZ_WEIGHTS_I32,
+    "logits": {torch.float32: _lib.AZ_LOGITS_F32, torch.bfloat16: _lib.AZ_LOGITS_BF16,
+               torch.float16: _lib.AZ_LOGITS_F16},
+    "weights": {torch.float32: _lib.AZ_WEIGHTS_F32, torch.int32: _lib.AZ_WEIGHTS_I32},
 }
 _IDS = {torch.int32: 0, torch.int64: 1}
+
+# os_az_rows and os_az_target, packed as C lays them out: for the smallest
+# batches a call costs what its checks cost, and a ctypes.Structure takes four
+# times as long to fill.
+_ROWS = struct.Struct("@PPqqqiifi")
+_TARGET = struct.Struct("@PPqqiiii")
+if _ROWS.size != _lib.AZ_ROWS_BYTES or _TARGET.size != _lib.AZ_TARGET_BYTES:
+  raise ImportError("os_az_rows / os_az_target are not laid out as their bindings")
+
+try:  # the current stream's handle, without a torch.cuda.Stream around it
+  _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:
+  def _raw_stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 class LogProbs(NamedTuple):
@@ -60,134 +73,147 @@ class LogProbs(NamedTuple):
 
 
 def _rows(logits, legal, temperature):
-  """The checked os_az_rows of a call; its tensors must outlive it."""
-  if logits.dtype not in _DTYPES:
+  """(packed os_az_rows, N, A, device index) of a call, checked; its tensors
+  must outlive it."""
+  dtype = _DTYPES.get(logits.dtype)
+  if dtype is None:
     raise ValueError("logits must be float32, bfloat16 or float16")
-  if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+  shape = logits.shape
+  if len(shape) != 2:
+    raise ValueError("logits must be [N, A] with unit column stride")
+  n, a = shape
+  ld, step = logits.stride()
+  if a < 1 or (step != 1 and a > 1):
     raise ValueError("logits must be [N, A] with unit column stride")
   if not logits.is_cuda:
     raise ValueError("logits must be on a GPU")
-  n, a = logits.shape
+  dev = logits.get_device()
   if a > _lib.AZ_MAX_ACTIONS:
     raise ValueError("more than %d actions" % _lib.AZ_MAX_ACTIONS)
-  t = float(temperature)
-  if not 1e-30 <= t <= 1e30:
+  if not 1e-30 <= temperature <= 1e30:
     raise ValueError("temperature must be in [1e-30, 1e30]")
-  r = _lib.AzRows(logits=logits.data_ptr(), num_rows=n, ld=logits.stride(0), num_actions=a,
-                  dtype=_DTYPES[logits.dtype], temperature=t)
+  mask = legal_ld = 0
   if legal is not None:
-    if legal.dtype not in (torch.uint8, torch.bool):
+    if legal.dtype is not torch.uint8 and legal.dtype is not torch.bool:
       raise ValueError("legal must be uint8 or bool")
-    if tuple(legal.shape) not in ((n, a), (a,)) or (a > 1 and legal.stride(-1) != 1):
-      raise ValueError("legal must be [N, A] or [A] with unit column stride")
-    if legal.device != logits.device:
+    if legal.shape == shape:
+      legal_ld, step = legal.stride()
+    elif legal.shape == (a,):
+      step, = legal.stride()
+    else:
+      raise ValueError("legal must be [N, A] or [A]")
+    if step != 1 and a > 1:
+      raise ValueError("legal must have unit column stride")
+    if legal.get_device() != dev:
       raise ValueError("legal must be on the logits' GPU")
-    r.legal = legal.data_ptr()
-    r.legal_ld = legal.stride(0) if legal.dim() == 2 else 0
-  return r
+    mask = legal.data_ptr()
+  return (_ROWS.pack(logits.data_ptr(), mask, n, ld, legal_ld, a, dtype, temperature, 0), n, a,
+          dev)
 
 
-def _like(what, x, logits, dtype, *shape):
-  """Checks an optional result or per-row tensor: contiguous, of this shape."""
-  if x is None:
-    return None
-  if x.dtype != dtype or tuple(x.shape) != shape or not x.is_contiguous():
+def _like(what, x, dev, dtype, *shape):
+  """The address of a result or per-row tensor: contiguous, of this shape."""
+  if x.dtype is not dtype or x.shape != shape or not x.is_contiguous():
     raise ValueError("%s must be contiguous %s %s" % (what, dtype, list(shape)))
-  if x.device != logits.device:
+  if x.get_device() != dev:
     raise ValueError("%s must be on the logits' GPU" % what)
   return x.data_ptr()
 
 
-def _actions(actions, logits):
+def _actions(actions, n, dev):
   """(address, wide) of the given actions, one a row."""
   if actions is None:
     return None, 0
-  if actions.dtype not in _IDS:
+  wide = _IDS.get(actions.dtype)
+  if wide is None:
     raise ValueError("actions must be int32 or int64")
-  return (_like("actions", actions, logits, actions.dtype, logits.shape[0]),
-          _IDS[actions.dtype])
+  return _like("actions", actions, dev, actions.dtype, n), wide
 
 
-def _target(target, target_actions, logits, kind):
-  """The checked os_az_target of a call."""
-  n, a = logits.shape
-  if kind not in ("logits", "weights"):
+def _target(target, target_actions, n, a, dev, kind):
+  """The packed os_az_target of a call, checked."""
+  kinds = _TARGETS.get(kind)
+  if kinds is None:
     raise ValueError("kind must be 'logits' or 'weights'")
-  if (kind, target.dtype) not in _TARGETS:
+  dtype = kinds.get(target.dtype)
+  if dtype is None:
     raise ValueError("target must be float32, bfloat16 or float16 logits, or float32 or int32 "
                      "weights")
   if target.requires_grad:
     raise ValueError("the target is not differentiated: detach() it")
-  if target.dim() != 2 or target.shape[0] != n or (target.shape[1] > 1 and target.stride(1) != 1):
+  shape = target.shape
+  if len(shape) != 2 or shape[0] != n:
     raise ValueError("target must be [N, K] with unit column stride")
-  k = target.shape[1]
+  k = shape[1]
+  ld, step = target.stride()
+  if step != 1 and k > 1:
+    raise ValueError("target must be [N, K] with unit column stride")
   if k > _lib.AZ_MAX_TARGETS:
     raise ValueError("more than %d listed actions" % _lib.AZ_MAX_TARGETS)
-  if target.device != logits.device:
+  if target.get_device() != dev:
     raise ValueError("target must be on the logits' GPU")
-  t = _lib.AzTarget(target=target.data_ptr(), target_ld=target.stride(0), k=k,
-                    type=_TARGETS[kind, target.dtype])
+  ids = ids_ld = wide = 0
   if target_actions is None:
     if k != a:
       raise ValueError("a target without target_actions must be [N, A]")
-    return t
-  if target_actions.dtype not in _IDS:
-    raise ValueError("target_actions must be int32 or int64")
-  if tuple(target_actions.shape) != (n, k) or (k > 1 and target_actions.stride(1) != 1):
-    raise ValueError("target_actions must be shaped as target, with unit column stride")
-  if target_actions.device != logits.device:
-    raise ValueError("target_actions must be on the logits' GPU")
-  t.actions = target_actions.data_ptr()
-  t.actions_ld = target_actions.stride(0)
-  t.wide = _IDS[target_actions.dtype]
-  return t
-
-
-def _grad_buffer(grad, logits):
-  n, a = logits.shape
-  if grad.dtype != logits.dtype or tuple(grad.shape) != (n, a):
-    raise ValueError("grad must have the logits' type and shape")
-  if grad.device != logits.device:
-    raise ValueError("grad must be on the logits' GPU")
-  if (a > 1 and grad.stride(1) != 1) or (n > 1 and grad.stride(0) < a):
-    raise ValueError("grad must have unit column stride and rows that do not overlap")
-  if n > 0:
-    size = grad.element_size()
-    g0, x0 = grad.data_ptr(), logits.data_ptr()
-    if (g0 < x0 + ((n - 1) * logits.stride(0) + a) * size
-        and x0 < g0 + ((n - 1) * grad.stride(0) + a) * size
-        and not _interleaved(grad, logits, a)):
-      raise ValueError("grad overlaps the logits")
-  return grad.data_ptr(), max(grad.stride(0), a)
-
-
-def _interleaved(grad, logits, a):
-  """Whether two tensors of one row stride are disjoint columns of it (the
-  halves of one buffer)."""
-  ld = logits.stride(0)
-  if grad.stride(0) != ld:
-    return False
-  off = (grad.data_ptr() - logits.data_ptr()) // grad.element_size() % ld
-  return off >= a and off + a <= ld
-
-
-def _launch(fn, logits, *args):
-  """Calls a C entry on the current stream of the logits' device."""
-  dev = logits.device
-  if dev.index != torch.cuda.current_device():
-    with torch.cuda.device(dev):
-      check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
   else:
-    check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+    wide = _IDS.get(target_actions.dtype)
+    if wide is None:
+      raise ValueError("target_actions must be int32 or int64")
+    if target_actions.shape != shape:
+      raise ValueError("target_actions must be shaped as target")
+    ids_ld, step = target_actions.stride()
+    if step != 1 and k > 1:
+      raise ValueError("target_actions must have unit column stride")
+    if target_actions.get_device() != dev:
+      raise ValueError("target_actions must be on the logits' GPU")
+    ids = target_actions.data_ptr()
+  return _TARGET.pack(ids, target.data_ptr(), ids_ld, ld, k, dtype, wide, 0)
 
 
-def _workspace(rows, top, logits):
-  n = lib.os_az_rows_workspace(ctypes.byref(rows), top)
+def _grad_buffer(grad, logits, n, a, dev):
+  """(address, row stride) of the caller's gradient buffer, checked."""
+  if grad.dtype is not logits.dtype or grad.shape != logits.shape:
+    raise ValueError("grad must have the logits' type and shape")
+  if grad.get_device() != dev:
+    raise ValueError("grad must be on the logits' GPU")
+  ld, step = grad.stride()
+  if (step != 1 and a > 1) or (ld < a and n > 1):
+    raise ValueError("grad must have unit column stride and rows that do not overlap")
+  ld = max(ld, a)
+  g0 = grad.data_ptr()
+  if n > 0:
+    size, x0, x_ld = grad.element_size(), logits.data_ptr(), logits.stride(0)
+    if (g0 < x0 + ((n - 1) * x_ld + a) * size and x0 < g0 + ((n - 1) * ld + a) * size):
+      # their extents meet: fine as disjoint columns of one buffer's rows
+      off = (g0 - x0) // size % ld
+      if x_ld != ld or off < a or off + a > ld:
+        raise ValueError("grad overlaps the logits")
+  return g0, ld
+
+
+def _launch(fn, dev, *args):
+  """Calls a C entry on the device's current stream."""
+  if dev == torch.cuda.current_device():
+    rc = fn(*args, _raw_stream(dev))
+  else:
+    with torch.cuda.device(dev):
+      rc = fn(*args, _raw_stream(dev))
+  if rc:
+    check(rc)
+
+
+def _workspace(rows, a, top, dev):
+  """(tensor to keep until the call, address, bytes): rows of few actions need
+  none (os_az_rows_workspace)."""
+  if a <= _lib.AZ_NO_WORKSPACE_ACTIONS:
+    return None, None, 0
+  n = lib.os_az_rows_workspace(rows, top)
   if n < 0:
     check(int(n))
   if n == 0:
     return None, None, 0
-  w = torch.empty(n, dtype=torch.uint8, device=logits.device)
+  w = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", dev))
   return w, w.data_ptr(), n
 
 
@@ -197,27 +223,26 @@ def logprobs_into(logits, entropy, logprob=None, actions=None, legal=None, top_a
   int64 and top_logprob float32 [N, top], stats float32 [N, 2] (what the
   gradient needs; optional).  logprob and actions go together, and so do the
   top pair."""
-  rows = _rows(logits, legal, temperature)
-  n = logits.shape[0]
-  act, wide = _actions(actions, logits)
+  rows, n, a, dev = _rows(logits, legal, temperature)
+  act, wide = _actions(actions, n, dev)
   if (logprob is None) != (actions is None):
     raise ValueError("logprob and actions go together")
   if (top_action is None) != (top_logprob is None):
     raise ValueError("top_action and top_logprob go together")
   if entropy is None:
     raise ValueError("entropy is needed")
-  top = 0
+  lp = None if logprob is None else _like("logprob", logprob, dev, _F32, n)
+  st = None if stats is None else _like("stats", stats, dev, _F32, n, 2)
+  top, ta, tl = 0, None, None
   if top_action is not None:
     if top_action.dim() != 2 or top_action.shape[1] > _lib.AZ_MAX_TOP:
       raise ValueError("top_action must be [N, top], top <= %d" % _lib.AZ_MAX_TOP)
     top = top_action.shape[1]
-  out = (_like("logprob", logprob, logits, torch.float32, n),
-         _like("entropy", entropy, logits, torch.float32, n),
-         _like("stats", stats, logits, torch.float32, n, 2), top,
-         _like("top_action", top_action, logits, torch.int64, n, top),
-         _like("top_logprob", top_logprob, logits, torch.float32, n, top))
-  keep, work, size = _workspace(rows, top, logits)
-  _launch(lib.os_az_logprobs_async, logits, ctypes.byref(rows), act, wide, *out, work, size)
+    ta = _like("top_action", top_action, dev, torch.int64, n, top)
+    tl = _like("top_logprob", top_logprob, dev, _F32, n, top)
+  h = _like("entropy", entropy, dev, _F32, n)
+  keep, work, size = _workspace(rows, a, top, dev)
+  _launch(lib.os_az_logprobs_async, dev, rows, act, wide, lp, h, st, top, ta, tl, work, size)
   del keep
 
 
@@ -227,21 +252,19 @@ def distill_into(logits, target, loss, target_entropy=None, target_actions=None,
   float32 [N, 2] (what the gradient needs; optional).  With `grad` (the logits'
   type and shape, any row stride) also the logits' gradient of
   (weight * loss).sum(); weight float32 [N], None: 1."""
-  rows = _rows(logits, legal, temperature)
-  n = logits.shape[0]
-  t = _target(target, target_actions, logits, kind)
+  rows, n, a, dev = _rows(logits, legal, temperature)
+  t = _target(target, target_actions, n, a, dev, kind)
   if loss is None:
     raise ValueError("loss is needed")
   if weight is not None and grad is None:
     raise ValueError("weight scales the gradient: it needs grad")
-  g, ld = (None, 0) if grad is None else _grad_buffer(grad, logits)
-  out = (_like("weight", weight, logits, torch.float32, n),
-         _like("loss", loss, logits, torch.float32, n),
-         _like("target_entropy", target_entropy, logits, torch.float32, n),
-         _like("stats", stats, logits, torch.float32, n, 2))
-  keep, work, size = _workspace(rows, 0, logits)
-  _launch(lib.os_az_distill_async, logits, ctypes.byref(rows), ctypes.byref(t), *out, g, ld, work,
-          size)
+  g, ld = (None, 0) if grad is None else _grad_buffer(grad, logits, n, a, dev)
+  w = None if weight is None else _like("weight", weight, dev, _F32, n)
+  out = _like("loss", loss, dev, _F32, n)
+  h = None if target_entropy is None else _like("target_entropy", target_entropy, dev, _F32, n)
+  st = None if stats is None else _like("stats", stats, dev, _F32, n, 2)
+  keep, work, size = _workspace(rows, a, 0, dev)
+  _launch(lib.os_az_distill_async, dev, rows, t, w, out, h, st, g, ld, work, size)
   del keep
 
 
@@ -251,22 +274,55 @@ def _per_row(g):
   return (None, 0) if g is None else (g.data_ptr(), g.stride(0))
 
 
+def _new_logprobs(logits, actions, legal, top, temperature, keep_stats):
+  """logprobs' results in new tensors, and the stats their gradient needs."""
+  rows, n, a, dev = _rows(logits, legal, temperature)
+  act, wide = _actions(actions, n, dev)
+  device = logits.device
+  entropy = torch.empty(n, dtype=_F32, device=device)
+  logprob = top_action = top_logprob = stats = lp = st = ta = tl = None
+  if actions is not None:
+    logprob = torch.empty(n, dtype=_F32, device=device)
+    lp = logprob.data_ptr()
+  if keep_stats:
+    stats = torch.empty(n, 2, dtype=_F32, device=device)
+    st = stats.data_ptr()
+  if top > 0:
+    top_action = torch.empty(n, top, dtype=torch.int64, device=device)
+    top_logprob = torch.empty(n, top, dtype=_F32, device=device)
+    ta, tl = top_action.data_ptr(), top_logprob.data_ptr()
+  keep, work, size = _workspace(rows, a, top, dev)
+  _launch(lib.os_az_logprobs_async, dev, rows, act, wide, lp, entropy.data_ptr(), st, top, ta, tl,
+          work, size)
+  del keep
+  return logprob, entropy, top_action, top_logprob, stats
+
+
+def _new_distill(logits, target, target_actions, legal, kind, temperature, keep_stats):
+  rows, n, a, dev = _rows(logits, legal, temperature)
+  t = _target(target, target_actions, n, a, dev, kind)
+  device = logits.device
+  loss = torch.empty(n, dtype=_F32, device=device)
+  entropy = torch.empty(n, dtype=_F32, device=device)
+  stats = st = None
+  if keep_stats:
+    stats = torch.empty(n, 2, dtype=_F32, device=device)
+    st = stats.data_ptr()
+  keep, work, size = _workspace(rows, a, 0, dev)
+  _launch(lib.os_az_distill_async, dev, rows, t, None, loss.data_ptr(), entropy.data_ptr(), st,
+          None, 0, work, size)
+  del keep
+  return loss, entropy, stats
+
+
 class _LogProbs(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, logits, actions, legal, top, temperature):
-    n = logits.shape[0]
-    f32 = dict(dtype=torch.float32, device=logits.device)
-    entropy = torch.empty(n, **f32)
-    stats = torch.empty(n, 2, **f32)
-    logprob = None if actions is None else torch.empty(n, **f32)
-    top_action = top_logprob = None
-    if top > 0:
-      top_action = torch.empty(n, top, dtype=torch.int64, device=logits.device)
-      top_logprob = torch.empty(n, top, **f32)
+    logprob, entropy, top_action, top_logprob, stats = _new_logprobs(
+        logits, actions, legal, top, temperature, True)
+    if top_action is not None:
       ctx.mark_non_differentiable(top_action)
-    logprobs_into(logits, entropy, logprob, actions, legal, top_action, top_logprob, temperature,
-                  stats)
     ctx.save_for_backward(logits, actions, legal, entropy, stats, top_action)
     ctx.temperature = temperature
     ctx.set_materialize_grads(False)
@@ -278,18 +334,16 @@ class _LogProbs(torch.autograd.Function):
     if g_logprob is None and g_entropy is None and g_top is None:
       return (None,) * 5
     logits, actions, legal, entropy, stats, top_action = ctx.saved_tensors
-    rows = _rows(logits, legal, ctx.temperature)
-    act, wide = _actions(actions, logits)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    top = 0
+    rows, n, a, dev = _rows(logits, legal, ctx.temperature)
+    act, wide = _actions(actions, n, dev)
+    grad = torch.empty(n, a, dtype=logits.dtype, device=logits.device)
+    top, ta, gt = 0, None, None
     if g_top is not None:
       g_top = g_top.contiguous()
-      top = g_top.shape[1]
-    _launch(lib.os_az_logprobs_grad_async, logits, ctypes.byref(rows), act, wide,
-            entropy.data_ptr(), stats.data_ptr(), top,
-            None if top == 0 else top_action.data_ptr(), *_per_row(g_logprob),
-            *_per_row(g_entropy), None if top == 0 else g_top.data_ptr(), grad.data_ptr(),
-            logits.shape[1])
+      top, ta, gt = g_top.shape[1], top_action.data_ptr(), g_top.data_ptr()
+    _launch(lib.os_az_logprobs_grad_async, dev, rows, act, wide, entropy.data_ptr(),
+            stats.data_ptr(), top, ta, *_per_row(g_logprob), *_per_row(g_entropy), gt,
+            grad.data_ptr(), a)
     return grad, None, None, None, None
 
 
@@ -297,11 +351,8 @@ class _Distill(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, logits, target, target_actions, legal, kind, temperature):
-    n = logits.shape[0]
-    f32 = dict(dtype=torch.float32, device=logits.device)
-    loss, entropy, stats = torch.empty(n, **f32), torch.empty(n, **f32), torch.empty(n, 2, **f32)
-    distill_into(logits, target, loss, entropy, target_actions, legal, kind, temperature,
-                 stats=stats)
+    loss, entropy, stats = _new_distill(logits, target, target_actions, legal, kind, temperature,
+                                        True)
     ctx.save_for_backward(logits, target, target_actions, legal, stats)
     ctx.kind, ctx.temperature = kind, temperature
     ctx.mark_non_differentiable(entropy)
@@ -314,12 +365,16 @@ class _Distill(torch.autograd.Function):
     if g_loss is None:
       return (None,) * 6
     logits, target, target_actions, legal, stats = ctx.saved_tensors
-    rows = _rows(logits, legal, ctx.temperature)
-    t = _target(target, target_actions, logits, ctx.kind)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _launch(lib.os_az_distill_grad_async, logits, ctypes.byref(rows), ctypes.byref(t),
-            *_per_row(g_loss), stats.data_ptr(), grad.data_ptr(), logits.shape[1])
+    rows, n, a, dev = _rows(logits, legal, ctx.temperature)
+    t = _target(target, target_actions, n, a, dev, ctx.kind)
+    grad = torch.empty(n, a, dtype=logits.dtype, device=logits.device)
+    _launch(lib.os_az_distill_grad_async, dev, rows, t, *_per_row(g_loss), stats.data_ptr(),
+            grad.data_ptr(), a)
     return grad, None, None, None, None, None
+
+
+def _differentiated(logits):
+  return logits.requires_grad and torch.is_grad_enabled()
 
 
 def logprobs(logits, actions=None, legal=None, top=0, temperature=1.0):
@@ -336,7 +391,9 @@ def logprobs(logits, actions=None, legal=None, top=0, temperature=1.0):
   top = int(top)
   if not 0 <= top <= _lib.AZ_MAX_TOP:
     raise ValueError("top must be in [0, %d]" % _lib.AZ_MAX_TOP)
-  return LogProbs(*_LogProbs.apply(logits, actions, legal, top, float(temperature)))
+  if _differentiated(logits):
+    return LogProbs(*_LogProbs.apply(logits, actions, legal, top, temperature))
+  return LogProbs(*_new_logprobs(logits, actions, legal, top, temperature, False)[:4])
 
 
 def distill(logits, target, target_actions=None, legal=None, kind="weights", temperature=1.0):
@@ -355,7 +412,9 @@ def distill(logits, target, target_actions=None, legal=None, kind="weights", tem
   The loss is 0 for a row without a target, +inf where an excluded action has
   mass, NaN where an action >= A is listed.  The gradient reaches the logits,
   not the target; an excluded action's is 0."""
-  return _Distill.apply(logits, target, target_actions, legal, kind, float(temperature))
+  if _differentiated(logits):
+    return _Distill.apply(logits, target, target_actions, legal, kind, temperature)
+  return _new_distill(logits, target, target_actions, legal, kind, temperature, False)[:2]
 
 
 def search_targets(out, device):
