@@ -420,7 +420,7 @@ struct Dense {
   }
 };
 
-// ---- rows of more than kTinyMax actions ----
+// ---- long rows ----
 
 template <int kOp>
 using ArgsOf = std::conditional_t<kOp == kLogprobs || kOp == kLogprobsTop, LogprobArgs,
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
   constexpr bool kEnt = kOp == kLogprobs || kOp == kLogprobsTop;
   constexpr bool kTarget = kOp == kDistill || kOp == kDistillFused || kOp == kDistillGrad;
   constexpr bool kSecond = kTop || kGrad;            // a second pass over the registers
-  constexpr int kHeld = kN == kFewChunks ? 8 : 1;    // target entries a lane keeps
+  constexpr int kHeld = kN == kFewChunks ? 4 : 1;    // target entries a lane keeps
   using Word = std::conditional_t<kE == 8, uint64_t, uint32_t>;  // a chunk's mask bytes
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   __shared__ float red[2][kMaxWaves][8];
@@ -515,8 +515,6 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     Mass mass{neg_inf(), 0.0f};
     float bad = 0.0f;
     Table tab{};
-    float* dq = nullptr;
-    bool in_order = false;  // dense LDS: an action listed twice
     if constexpr (kTarget) {
       const int k = g.t.k;
       const auto take = [&](Entry e) {
@@ -543,39 +541,13 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
       for (int i = 0; i < kHeld; ++i)
         if (i * bd < k && eid[i] >= 0) ex[i] = logit<T>(a, r, eid[i]);
       if constexpr (kGrad) {
-        if (kN == kFewChunks && nw == 1) {
-          // One wave: the row's weights as an array in LDS.  Each entry leaves
-          // its number; one that finds another's shares its action.
-          dq = reinterpret_cast<float*>(dyn);
-          int* const tag = reinterpret_cast<int*>(dyn);
-          if (g.t.ids != nullptr) {
-            const auto each = [&](auto f) {
-#pragma unroll
-              for (int i = 0; i < kHeld; ++i)
-                if (i * 64 < k && eid[i] >= 0) f(eid[i], tid + i * 64);
-              for (int j = tid + kHeld * 64; j < k; j += 64) {
-                const int64_t id = get_id(g.t.ids, g.t.wide, r * g.t.ids_ld + j);
-                if (id >= 0 && id < a.v) f(static_cast<int>(id), j);
-              }
-            };
-            each([&](int id, int j) { tag[id] = j; });
-            __syncthreads();
-            int clash = 0;
-            each([&](int id, int j) { clash |= tag[id] != j; });
-            in_order = __ballot(clash) != 0;
-            __syncthreads();
-          }
-          for (int i = tid; i < a.v; i += 64) dq[i] = 0.0f;
-          __syncthreads();
-        } else {
-          unsigned char* const base = dyn + static_cast<size_t>(par) * g.hash * 12;
-          tab.key = reinterpret_cast<int32_t*>(base);
-          tab.w = reinterpret_cast<float*>(base + static_cast<size_t>(g.hash) * 4);
-          tab.x = reinterpret_cast<float*>(base + static_cast<size_t>(g.hash) * 8);
-          tab.mask = g.hash - 1;
-          table_clear(tab, tid, bd);
-          if (tid == 0) twice[par] = 0;
-        }
+        unsigned char* const base = dyn + static_cast<size_t>(par) * g.hash * 12;
+        tab.key = reinterpret_cast<int32_t*>(base);
+        tab.w = reinterpret_cast<float*>(base + static_cast<size_t>(g.hash) * 4);
+        tab.x = reinterpret_cast<float*>(base + static_cast<size_t>(g.hash) * 8);
+        tab.mask = g.hash - 1;
+        table_clear(tab, tid, bd);
+        if (tid == 0) twice[par] = 0;
       }
     }
 
@@ -783,13 +755,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
           }
         }
         if constexpr (kGrad) {
-          if (id >= 0 && x > neg_inf()) {
-            if (dq != nullptr) {
-              if (!in_order) dq[id] = -scale * q;
-            } else if (id >= lo && id < lo + len) {
-              if (!table_put(tab, id, -scale * q, x)) twice[par] = 1;
-            }
-          }
+          if (id >= lo && id < lo + len && x > neg_inf())
+            if (!table_put(tab, id, -scale * q, x)) twice[par] = 1;
         }
       };
 #pragma unroll
@@ -799,20 +766,6 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
         const Entry e = target_entry(g.t, r, j);
         const int id = e.id < 0 || e.id >= a.v ? -1 : static_cast<int>(e.id);
         use(id, e.z, id < 0 ? neg_inf() : logit<T>(a, r, id));
-      }
-      if constexpr (kGrad) {
-        if (dq != nullptr) {
-          __syncthreads();
-          if (in_order) {
-            if (tid == 0)
-              for (int j = 0; j < g.t.k; ++j) {
-                const Entry e = target_entry(g.t, r, j);
-                if (e.id >= 0 && e.id < a.v && logit<T>(a, r, e.id) > neg_inf())
-                  dq[e.id] -= scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
-              }
-            __syncthreads();
-          }
-        }
       }
       if constexpr (kOp != kDistillGrad) {
         ce = fold64(ce, Add{});
@@ -902,12 +855,6 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
 #pragma unroll
             for (int j = 0; j < kE; ++j) y[j] = x[j] == neg_inf() ? 0.0f : y[j];
           }
-          if constexpr (kTarget && kN == kFewChunks) {
-            if (dq != nullptr) {
-#pragma unroll
-              for (int j = 0; j < kE; ++j) y[j] += dq[oc + j];
-            }
-          }
           if (o + kE <= len) {
             store_at<T>(gb + o, pack<T>(y));
           } else if (o < len) {
@@ -924,28 +871,24 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
         gb[id - lo] = static_cast<T>(dn.template at<kLog>(x) + w);
       };
       if constexpr (kTarget) {
-        if (dq == nullptr) {
+        __syncthreads();
+        if (twice[par] != 0) {
           __syncthreads();
-          if (twice[par] != 0) {
-            __syncthreads();
-            table_clear(tab, tid, bd);
-            __syncthreads();
-            if (tid == 0)
-              for (int j = 0; j < g.t.k; ++j) {
-                const Entry e = target_entry(g.t, r, j);
-                if (e.id < lo || e.id >= lo + len) continue;
-                const float x = logit<T>(a, r, e.id);
-                if (x > neg_inf())
-                  table_add(tab, static_cast<int>(e.id),
-                            -scale * (target_mass(g.t, a.c, e.z, mass.z) * inv), x);
-              }
-            __syncthreads();
-          }
-          for (int i = tid; i <= tab.mask; i += bd)
-            if (tab.key[i] >= 0) fix(tab.key[i], tab.w[i], tab.x[i]);
-        } else {
-          __syncthreads();  // dq is the next row's
+          table_clear(tab, tid, bd);
+          __syncthreads();
+          if (tid == 0)
+            for (int j = 0; j < g.t.k; ++j) {
+              const Entry e = target_entry(g.t, r, j);
+              if (e.id < lo || e.id >= lo + len) continue;
+              const float x = logit<T>(a, r, e.id);
+              if (x > neg_inf())
+                table_add(tab, static_cast<int>(e.id),
+                          -scale * (target_mass(g.t, a.c, e.z, mass.z) * inv), x);
+            }
+          __syncthreads();
         }
+        for (int i = tid; i <= tab.mask; i += bd)
+          if (tab.key[i] >= 0) fix(tab.key[i], tab.w[i], tab.x[i]);
       } else {
         __syncthreads();
         const bool mine = act >= lo && act < lo + len && act_x > neg_inf();
@@ -974,6 +917,404 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
             if (tab.key[i] >= 0) fix(tab.key[i], tab.w[i], tab.x[i]);
         }
       }
+    }
+  }
+}
+
+// ---- rows of up to four chunks a lane: a wave each ----
+
+// The largest of one value a lane below which fewer than k of 64 lanes (k <= 8:
+// of 16 groups of 4, for a quarter of the work) lie above it: `top`'s bound.
+__device__ __forceinline__ float kth_value(float v, int k) {
+  int rank = 0;
+  if (k <= 8) {
+    float q = v;
+    q = fmaxf(q, __shfl_xor(q, 16));
+    q = fmaxf(q, __shfl_xor(q, 32));
+    const auto above = [&](float o) { rank += o > q ? 1 : 0; };
+    above(dpp<0x121>(q));
+    above(dpp<0x122>(q));
+    above(dpp<0x123>(q));
+    above(dpp<0x124>(q));
+    above(dpp<0x125>(q));
+    above(dpp<0x126>(q));
+    above(dpp<0x127>(q));
+    above(dpp<0x128>(q));
+    above(dpp<0x129>(q));
+    above(dpp<0x12A>(q));
+    above(dpp<0x12B>(q));
+    above(dpp<0x12C>(q));
+    above(dpp<0x12D>(q));
+    above(dpp<0x12E>(q));
+    above(dpp<0x12F>(q));
+    v = q;
+  } else {
+#pragma unroll 8
+    for (int j = 0; j < 64; ++j) rank += lane_at(v, j) > v ? 1 : 0;
+  }
+  // of the values with fewer than k above them, the least
+  return -fold64(rank < k ? -v : neg_inf(), Max{});
+}
+
+// kC chunks a lane, the values in registers as floats; the next row's chunks
+// are under way while a row is worked on.  No barrier is needed: what goes
+// through LDS stays within the wave, whose accesses are in order (fence() keeps
+// the compiler to it).
+template <class T, bool kMask, int kC, int kOp>
+__global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
+  constexpr int kE = kPer<T>, kX = kC * kE;
+  constexpr bool kSums = kOp != kLogprobsGrad && kOp != kDistillGrad;
+  constexpr bool kGrad = kOp == kLogprobsGrad || kOp == kDistillGrad || kOp == kDistillFused;
+  constexpr bool kLp = kOp == kLogprobs || kOp == kLogprobsTop;
+  constexpr bool kTarget = kOp == kDistill || kOp == kDistillFused || kOp == kDistillGrad;
+  constexpr int kHeld = 8;  // target entries a lane keeps in registers
+  using Word = std::conditional_t<kE == 8, uint64_t, uint32_t>;
+  // The row's values, then its listed weights: chunk (t, lane) at
+  // (t * 64 + lane) * kE, the row's last actions where their chunk has them.
+  __shared__ __attribute__((aligned(16))) float row[kTarget || kGrad ? 64 * kX : 1];
+  __shared__ uint64_t cand[kOp == kLogprobsTop ? 64 : 1];
+  const int lane = threadIdx.x;
+  const int last = a.v - kE;
+  const auto fence = [] { __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront"); };
+
+  u32x4 raw[kC];
+  Word mk[kMask ? kC : 1];
+  const auto load = [&](int64_t r) {
+    const T* const x = static_cast<const T*>(a.x) + r * a.ld;
+    const uint8_t* const legal = kMask ? a.legal + r * a.lld : nullptr;
+#pragma unroll
+    for (int t = 0; t < kC; ++t) {
+      const int oc = min((t * 64 + lane) * kE, last);
+      raw[t] = load_at<T, u32x4>(x + oc);
+      if constexpr (kMask) mk[t] = load_at<uint8_t, Word>(legal + oc);
+    }
+  };
+  // Where an action is in `row`: the last, shifted chunk holds those from
+  // `edge` on.
+  const int edge = a.v / kE * kE, shift = (kE - a.v % kE) % kE;
+  const auto slot = [&](int id) { return id + (id >= edge ? shift : 0); };
+
+  load(blockIdx.x);
+  for (int64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
+    // -- the row's values --
+    int me = lane;  // (renewed: offsets are cheaper computed than kept)
+    renew(me);
+    float x[kX];
+#pragma unroll
+    for (int t = 0; t < kC; ++t) {
+      float v[kE];
+      unpack<T>(raw[t], v);
+#pragma unroll
+      for (int j = 0; j < kE; ++j) x[t * kE + j] = v[j];
+      if constexpr (kMask) {
+#pragma unroll
+        for (int j = 0; j < kE; ++j)
+          if (((mk[t] >> (8 * j)) & 0xFF) == 0) x[t * kE + j] = neg_inf();
+      }
+      if (t >= kC / 2) {  // (the first half is full: fewer chunks would do else)
+        const int o = (t * 64 + me) * kE, drop = o - min(o, last);
+#pragma unroll
+        for (int j = 0; j < kE; ++j)
+          if (j < drop) x[t * kE + j] = neg_inf();
+      }
+    }
+    // -- what else the row needs from memory, ahead of the next row's loads --
+    int64_t given = -1;
+    float given_x = neg_inf();
+    if constexpr (kLp || kOp == kLogprobsGrad) {
+      if (g.actions != nullptr) given = get_id(g.actions, g.wide, r);
+      if (given >= 0 && given < a.v) given_x = logit<T>(a, r, given);
+    }
+    int eid[kTarget ? kHeld : 1];
+    float ez[kTarget ? kHeld : 1];
+    Mass mass{neg_inf(), 0.0f};
+    float bad = 0.0f;
+    const auto entry_id = [&](const Entry& e) {
+      return e.id < 0 || e.id >= a.v ? -1 : static_cast<int>(e.id);
+    };
+    if constexpr (kTarget) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        eid[i] = -1;
+        ez[i] = neg_inf();
+        if (i * 64 < g.t.k && lane + i * 64 < g.t.k) {
+          const Entry e = target_entry(g.t, r, lane + i * 64);
+          if (e.id >= a.v) bad = 1.0f;
+          eid[i] = entry_id(e);
+          ez[i] = e.z;
+        }
+      }
+    }
+    if (r + gridDim.x < a.n) load(r + gridDim.x);
+
+    // -- the sums --
+    float m, l, mean = 0.0f, lane_max = neg_inf();
+    if constexpr (kSums) {
+#pragma unroll
+      for (int i = 0; i < kX; ++i) lane_max = fmaxf(lane_max, x[i]);
+      m = fold64(lane_max, Max{});
+      if (m == neg_inf()) m = 0.0f;  // empty, or only NaN
+      float s = 0.0f, u = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kX; ++i) {
+        const float d = (x[i] - m) * a.c;
+        const float e = exp2_(d);
+        s += e;
+        if constexpr (kLp) u = fmaf(e, fmaxf(d, kFloor), u);
+      }
+      s = fold64(s, Add{});
+      l = s == 0.0f ? 0.0f : log2f(s);
+      if constexpr (kLp) mean = s == 0.0f ? 0.0f : fold64(u, Add{}) / s;
+    } else {
+      m = g.stats[2 * r];
+      l = g.stats[2 * r + 1];
+    }
+
+    if constexpr (kLp) {
+      if (lane == 0) {
+        g.entropy[r] = kLn2 * (l - mean);
+        if (g.stats != nullptr) {
+          g.stats[2 * r] = m;
+          g.stats[2 * r + 1] = l;
+        }
+        if (g.actions != nullptr)
+          g.logprob[r] = given < 0 ? 0.0f
+                         : given >= a.v ? __builtin_nanf("")
+                                        : log_p(a, given_x, m, l);
+      }
+    }
+    if constexpr (kOp == kLogprobsTop) {
+      // Everything from a lower bound of the top-th largest value on, listed
+      // (usually a few more than `top`) and ranked by counting.
+      const bool odd = l != l;
+      const auto put = [&](int rank, uint64_t key) {
+        g.top_action[r * g.top + rank] = key == 0 ? -1 : static_cast<int64_t>(key_index(key));
+        g.top_logprob[r * g.top + rank] =
+            odd ? l : key == 0 ? neg_inf() : log_p(a, key_value(key), m, l);
+      };
+      const float bound = fmaxf(kth_value(lane_max, g.top), kLowest);
+      int found = 0;
+      renew(me);
+      if (!odd) {
+#pragma unroll
+        for (int i = 0; i < kX; ++i) {
+          const uint64_t hit = __ballot(x[i] >= bound);
+          if (hit != 0) {
+            const int at = found + __builtin_amdgcn_mbcnt_hi(
+                static_cast<uint32_t>(hit >> 32),
+                __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hit), 0));
+            const int o = (i / kE * 64 + me) * kE;
+            if (x[i] >= bound && at < 64)
+              cand[at] = top_key(x[i], static_cast<uint32_t>(min(o, last) + i % kE));
+            found += __builtin_popcountll(hit);
+          }
+        }
+      }
+      if (found <= 64) {
+        fence();
+        const uint64_t key = lane < found ? cand[lane] : 0;
+        int rank = 0;
+        for (int j = 0; j < found; ++j) rank += cand[j] > key ? 1 : 0;
+        if (lane < found && rank < g.top) put(rank, key);
+        if (lane >= found && lane < g.top) put(lane, 0);
+        fence();
+      } else {
+        // Equal values at the bound: one round over the registers for each.
+        uint64_t prev = ~0ull;
+        for (int k = 0; k < g.top; ++k) {
+          uint64_t best = 0;
+          renew(me);
+#pragma unroll
+          for (int i = 0; i < kX; ++i) {
+            renew(x[i]);
+            const int o = (i / kE * 64 + me) * kE;
+            const uint64_t key = top_key(x[i], static_cast<uint32_t>(min(o, last) + i % kE));
+            if (x[i] > neg_inf() && key < prev && key > best) best = key;
+          }
+          best = fold64_max(best);
+          if (lane == 0) put(k, best);
+          prev = best;
+        }
+      }
+    }
+
+    // -- the listed entries --
+    Dense dn{m, l, a.c, 0.0f, 0.0f};
+    const auto clear = [&] {
+#pragma unroll
+      for (int t = 0; t < kX / 4; ++t)
+        *reinterpret_cast<u32x4*>(row + (t * 64 + lane) * 4) = u32x4{0, 0, 0, 0};
+    };
+    [[maybe_unused]] int* const tag = reinterpret_cast<int*>(row);
+    if constexpr (kTarget) {
+      const int k = g.t.k;
+      // f(id, z, number, i) for each of this lane's entries
+      const auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+          if (i * 64 < k) f(eid[i], ez[i], lane + i * 64);
+        for (int j = lane + kHeld * 64; j < k; j += 64) {
+          const Entry e = target_entry(g.t, r, j);
+          f(entry_id(e), e.z, j);
+        }
+      };
+      for (int j = lane + kHeld * 64; j < k; j += 64)
+        if (target_entry(g.t, r, j).id >= a.v) bad = 1.0f;
+      bool clash = false;
+      each([&](int id, float z, int j) {
+        mass_add(g.t, a.c, z, mass);
+        if (kGrad && g.t.ids != nullptr && id >= 0) tag[slot(id)] = j;
+      });
+      if constexpr (kGrad) {
+        // an entry that finds another's number shares its action
+        if (g.t.ids != nullptr) {
+          fence();
+          int c = 0;
+          each([&](int id, float z, int j) {
+            if (id >= 0) c |= tag[slot(id)] != j;
+          });
+          clash = __ballot(c) != 0;
+          fence();
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < kC; ++t)
+#pragma unroll
+        for (int j = 0; j < kE; ++j) row[(t * 64 + lane) * kE + j] = x[t * kE + j];
+      fence();
+      mass = mass_fold(g.t, a.c, mass, [](float z) { return fold64(z, Max{}); },
+                       [](float z) { return fold64(z, Add{}); });
+      bad = fold64(bad, Max{});
+      const float inv = mass.s == 0.0f ? 0.0f : 1.0f / mass.s;
+      float scale = 0.0f, ce = 0.0f, h = 0.0f;
+      if constexpr (kGrad) {
+        scale = (g.weight != nullptr ? g.weight[r * g.weight_stride] : 1.0f) * a.inv_t;
+        dn.f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
+      }
+      float ew[kGrad ? kHeld : 1];  // the weights, until the values are read
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        if (i * 64 < k) {
+          const float q = target_mass(g.t, a.c, ez[i], mass.z) * inv;
+          const float xi = eid[i] >= 0 ? row[slot(eid[i])] : neg_inf();
+          if constexpr (kOp != kDistillGrad) {
+            if (q != 0.0f) {
+              if (eid[i] >= 0) ce -= q * log_p(a, xi, m, l);
+              h -= q * (kLn2 * log2f(q));
+            }
+          }
+          if constexpr (kGrad) {
+            ew[i] = -scale * q;
+            if (!(xi > neg_inf())) eid[i] = -1;
+          }
+        }
+      }
+      for (int j = lane + kHeld * 64; j < k; j += 64) {
+        const Entry e = target_entry(g.t, r, j);
+        const int id = entry_id(e);
+        const float q = target_mass(g.t, a.c, e.z, mass.z) * inv;
+        if constexpr (kOp != kDistillGrad) {
+          if (q != 0.0f) {
+            if (id >= 0) ce -= q * log_p(a, row[slot(id)], m, l);
+            h -= q * (kLn2 * log2f(q));
+          }
+        }
+      }
+      if constexpr (kOp != kDistillGrad) {
+        ce = fold64(ce, Add{});
+        h = fold64(h, Add{});
+        if (lane == 0) {
+          g.loss[r] = bad != 0.0f ? __builtin_nanf("") : ce;
+          if (g.tent != nullptr) g.tent[r] = h;
+          if (g.stats != nullptr) {
+            g.stats[2 * r] = m;
+            g.stats[2 * r + 1] = l;
+          }
+        }
+      }
+      fence();
+      if constexpr (kGrad) {
+        clear();
+        fence();
+        if (!clash) {
+#pragma unroll
+          for (int i = 0; i < kHeld; ++i)
+            if (i * 64 < k && eid[i] >= 0) row[slot(eid[i])] = ew[i];
+          for (int j = lane + kHeld * 64; j < k; j += 64) {
+            const Entry e = target_entry(g.t, r, j);
+            const int id = entry_id(e);
+            if (id >= 0 && logit<T>(a, r, id) > neg_inf())
+              row[slot(id)] = -scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
+          }
+        } else if (lane == 0) {  // in list order
+          for (int j = 0; j < k; ++j) {
+            const Entry e = target_entry(g.t, r, j);
+            const int id = entry_id(e);
+            if (id >= 0 && logit<T>(a, r, id) > neg_inf())
+              row[slot(id)] -= scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
+          }
+        }
+        fence();
+      }
+    }
+    if constexpr (kOp == kLogprobsGrad) {
+      const bool in = g.gl != nullptr && given >= 0 && given < a.v;
+      const float gl = in ? g.gl[r * g.gls] : 0.0f;
+      float sum = g.gl != nullptr && given >= a.v ? __builtin_nanf("") : gl;
+      clear();
+      fence();
+      if (g.top > 0) {
+        int64_t ti = -1;
+        float gt = 0.0f;
+        if (lane < g.top) {
+          ti = g.top_action[r * g.top + lane];
+          if (ti >= a.v) ti = -1;
+          if (ti >= 0) gt = g.gt[r * g.top + lane];
+        }
+        sum += fold64(gt, Add{});
+        if (ti >= 0) tag[slot(static_cast<int>(ti))] = lane;
+        fence();
+        const bool clash = __ballot(ti >= 0 && tag[slot(static_cast<int>(ti))] != lane) != 0;
+        fence();
+        if (ti >= 0) row[slot(static_cast<int>(ti))] = clash ? 0.0f : gt * a.inv_t;
+        fence();
+        if (clash && lane == 0)
+          for (int j = 0; j < g.top; ++j) {
+            const int64_t id = g.top_action[r * g.top + j];
+            if (id >= 0 && id < a.v) row[slot(static_cast<int>(id))] += g.gt[r * g.top + j] * a.inv_t;
+          }
+        fence();
+      }
+      if (lane == 0 && in) row[slot(static_cast<int>(given))] += gl * a.inv_t;
+      fence();
+      const float gh = g.gh != nullptr ? g.gh[r * g.ghs] : 0.0f;
+      dn.f0 = -(sum + (gh != 0.0f ? gh * g.entropy[r] : 0.0f)) * a.inv_t;
+      dn.f1 = -gh * kLn2 * a.inv_t;
+    }
+
+    // -- the gradient --
+    if constexpr (kGrad) {
+      T* const gb = static_cast<T*>(g.grad) + r * g.grad_ld;
+      renew(me);
+#pragma unroll
+      for (int t = 0; t < kC; ++t) {
+        float y[kE];
+#pragma unroll
+        for (int j = 0; j < kE; ++j) {
+          const float v = x[t * kE + j];
+          y[j] = dn.template at<kOp == kLogprobsGrad>(v) + row[(t * 64 + me) * kE + j];
+          if (v == neg_inf()) y[j] = 0.0f;
+        }
+        const int o = (t * 64 + me) * kE;
+        if (t < kC / 2 || o + kE <= a.v) {
+          store_at<T>(gb + o, pack<T>(y));
+        } else if (o < a.v) {
+#pragma unroll
+          for (int j = 0; j < kE; ++j)
+            if (last + j >= o) gb[last + j] = static_cast<T>(y[j]);
+        }
+      }
+      fence();
     }
   }
 }
@@ -1298,7 +1639,8 @@ struct Launch {
   Rows a;
   Parts pt;
   dim3 grid;
-  int waves;       // 0: k_tiny
+  int waves;       // 0: k_tiny; 1 with `wave` chunks: k_wave
+  int wave;        // chunks a lane of k_wave (1, 2 or 4), 0: k_rows
   bool few;        // kFewChunks chunks a lane
   unsigned lds;    // dynamic, bytes
   hipStream_t stream;

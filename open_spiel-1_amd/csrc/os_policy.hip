@@ -25,6 +25,7 @@ static_assert(OS_AZ_NO_WORKSPACE_ACTIONS * 4 <= 4 * kWaveFew);
 
 struct Plan {
   int waves;  // 0: k_tiny
+  int wave;   // chunks a lane of k_wave, 0: k_rows
   bool few;
   Parts pt;
   dim3 grid;
@@ -51,19 +52,29 @@ dim3 row_grid(int64_t n, const Plan& p, int resident) {
   return dim3(static_cast<unsigned>(up(n, rounds)), static_cast<unsigned>(p.pt.parts));
 }
 
-Plan tiny_plan(int64_t n) {
-  Plan p{0, true, Parts{1, 0}, dim3(1)};
-  p.grid = dim3(static_cast<unsigned>(std::min<int64_t>(up(n, kTinyRows), kCus * 8)));
-  return p;
+// Rows of at most four chunks a lane: 16 lanes or a wave each.
+bool short_rows(const Rows& a, int size, Plan* p) {
+  const int64_t bytes = int64_t{a.v} * size;
+  if (bytes > kWaveFew && a.v > kTinyMax) return false;
+  p->pt = Parts{1, a.v};
+  p->few = true;
+  if (a.v <= kTinyMax) {
+    p->grid = dim3(static_cast<unsigned>(std::min<int64_t>(up(a.n, kTinyRows), kCus * 8)));
+    return true;
+  }
+  p->waves = 1;
+  p->wave = bytes <= kKib ? 1 : bytes <= 2 * kKib ? 2 : 4;
+  p->grid = row_grid(a.n, *p, 24);
+  return true;
 }
 
 int64_t wave_bytes(const Rows& a) { return (a.legal ? kMaskChunks : kChunks) * kKib; }
 
 // Kernels that need the row's sums.
 Plan sums_plan(const Rows& a, int size) {
-  if (a.v <= kTinyMax) return tiny_plan(a.n);
-  const int64_t bytes = int64_t{a.v} * size, wave = wave_bytes(a);
   Plan p{};
+  if (short_rows(a, size, &p)) return p;
+  const int64_t bytes = int64_t{a.v} * size, wave = wave_bytes(a);
   int64_t parts = 1;
   if (bytes <= 4 * kWaveFew) {
     p.few = true;
@@ -83,9 +94,9 @@ Plan sums_plan(const Rows& a, int size) {
 
 // Gradients from known sums: parts are free, and small ones overlap better.
 Plan grad_plan(const Rows& a, int size) {
-  if (a.v <= kTinyMax) return tiny_plan(a.n);
-  const int64_t bytes = int64_t{a.v} * size;
   Plan p{};
+  if (short_rows(a, size, &p)) return p;
+  const int64_t bytes = int64_t{a.v} * size;
   p.few = bytes <= 4 * kWaveFew;
   p.pt = split(a.v, up(bytes, 64 * kKib));
   p.waves = static_cast<int>(up(int64_t{p.pt.part} * size, p.few ? kWaveFew : wave_bytes(a)));
@@ -96,7 +107,7 @@ Plan grad_plan(const Rows& a, int size) {
 int type_size(int dtype) { return dtype == OS_AZ_F32 ? 4 : 2; }
 
 Launch launch(const Rows& a, const Plan& p, void* stream) {
-  return Launch{a, p.pt, p.grid, p.waves, p.few, 0, static_cast<hipStream_t>(stream)};
+  return Launch{a, p.pt, p.grid, p.waves, p.wave, p.few, 0, static_cast<hipStream_t>(stream)};
 }
 
 // Each part's sums and top keys, and the rows' stats where a caller wants none.
@@ -105,14 +116,9 @@ int64_t workspace_bytes_of(const Rows& a, const Plan& p, int top) {
   return a.n * (p.pt.parts * (static_cast<int64_t>(sizeof(PartSums)) + 8 * int64_t{top}) + 8);
 }
 
-// The LDS of a target's listed weights: an array over the row where one wave
-// has it, else two tables (a row's and the next one's).
-void target_lds(const Rows& a, const Plan& p, DistillArgs* g, Launch* c) {
-  if (p.waves == 0) return;
-  if (p.few && p.waves == 1) {
-    c->lds = static_cast<unsigned>(a.v) * 4;
-    return;
-  }
+// The LDS of k_rows' tables of listed weights: a row's and the next one's.
+void target_lds(const Plan& p, DistillArgs* g, Launch* c) {
+  if (p.waves == 0 || p.wave != 0) return;
   g->hash = 64;
   while (g->hash < 2 * g->t.k) g->hash *= 2;
   c->lds = static_cast<unsigned>(g->hash) * 24;
@@ -262,7 +268,7 @@ int os_az_logprobs_grad_async(const os_az_rows* rows, const void* actions, int32
                             g_top,      grad,             grad_ld};
     return by_dtype(rows->dtype, [&](auto k) {
       Launch c = launch(a, p, hip_stream);
-      c.lds = p.waves > 0 && top > 0 ? 2 * 128 * 12 : 0;
+      c.lds = p.waves > 0 && p.wave == 0 && top > 0 ? 2 * 128 * 12 : 0;
       k.rows(c, g);
     });
   });
@@ -290,7 +296,7 @@ int os_az_distill_async(const os_az_rows* rows, const os_az_target* target, cons
     return by_dtype(rows->dtype, [&](auto k) {
       Launch c = launch(a, p, hip_stream);
       if (!parts) {
-        if (grad) target_lds(a, p, &g, &c);
+        if (grad) target_lds(p, &g, &c);
         k.rows(c, grad ? kDistillFused : kDistill, g);
         return;
       }
@@ -304,7 +310,7 @@ int os_az_distill_async(const os_az_rows* rows, const os_az_target* target, cons
       if (!grad) return;
       const Plan q = grad_plan(a, size);
       Launch d = launch(a, q, hip_stream);
-      target_lds(a, q, &g, &d);
+      target_lds(q, &g, &d);
       k.rows(d, kDistillGrad, g);
     });
   });
@@ -327,7 +333,7 @@ int os_az_distill_grad_async(const os_az_rows* rows, const os_az_target* target,
                   grad, grad_ld, 0};
     return by_dtype(rows->dtype, [&](auto k) {
       Launch c = launch(a, p, hip_stream);
-      target_lds(a, p, &g, &c);
+      target_lds(p, &g, &c);
       k.rows(c, kDistillGrad, g);
     });
   });

@@ -12,6 +12,20 @@ void launch_rows(const Launch& c, const G& g) {
     hipLaunchKernelGGL((k_tiny<T, kOp>), c.grid, dim3(kTinyBlock), 0, c.stream, c.a, g);
     return;
   }
+  if (c.wave != 0) {
+    const auto go = [&](auto mask) {
+      constexpr bool kMask = decltype(mask)::value;
+      if (c.wave == 1)
+        hipLaunchKernelGGL((k_wave<T, kMask, 1, kOp>), c.grid, dim3(64), 0, c.stream, c.a, g);
+      else if (c.wave == 2)
+        hipLaunchKernelGGL((k_wave<T, kMask, 2, kOp>), c.grid, dim3(64), 0, c.stream, c.a, g);
+      else
+        hipLaunchKernelGGL((k_wave<T, kMask, 4, kOp>), c.grid, dim3(64), 0, c.stream, c.a, g);
+    };
+    if (c.a.legal != nullptr) go(std::true_type{});
+    else go(std::false_type{});
+    return;
+  }
   const dim3 block(64 * c.waves);
   if (c.a.legal != nullptr) {
     if (c.few)
