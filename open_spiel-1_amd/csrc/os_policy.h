@@ -38,7 +38,10 @@ constexpr float kLn2 = 0.69314718055994530942f;
 // d below this is e = 0 in f32 (2^-149 is the least subnormal): keeps 0 * -inf
 // out of the sums.
 constexpr float kFloor = -160.0f;
-// The running maximum's start: finite, so that (-inf) - m is never NaN.
+// Rows whose maximum times c is further out than this ("wild") take the plain
+// form 2^((x - m) c): beyond it the rounding of m c alone would be over half a
+// unit of the exponent.
+constexpr float kWild = 16777216.0f;
 constexpr float kLowest = -3.4028234663852886e38f;
 constexpr int kTinyMax = 64;       // rows of up to this many actions: 16 lanes each
 constexpr int kMaxWaves = 16;
@@ -130,6 +133,10 @@ template <class V>
 __device__ __forceinline__ void renew(V& x) {
   asm volatile("" : "+v"(x));
 }
+__device__ __forceinline__ int renewed_scalar(int x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_huge_valf(); }
 __device__ __forceinline__ float exp2_(float d) { return __builtin_amdgcn_exp2f(d); }
@@ -214,6 +221,17 @@ __device__ __forceinline__ float log_p(const Rows& a, float x, float m, float l)
   return fmaf(x - m, a.inv_t, -l * kLn2);
 }
 
+// The largest of a chunk's values: v_maximum3_f32, which needs no quieting of
+// its operands (a NaN passes through: callers take it for none).
+template <int kE>
+__device__ __forceinline__ float largest(const float (&x)[kE]) {
+  const auto mx = [](float p, float q) { return __builtin_elementwise_maximum(p, q); };
+  float m = mx(mx(x[0], x[1]), x[2]);
+#pragma unroll
+  for (int j = 3; j + 1 < kE; j += 2) m = mx(mx(m, x[j]), x[j + 1]);
+  return mx(m, x[kE - 1]);
+}
+
 // ---- reductions ----
 
 template <int kCtrl>
@@ -251,17 +269,17 @@ __device__ __forceinline__ float fold64(float v, F f) {
   return f(f(lane_at(v, 0), lane_at(v, 16)), f(lane_at(v, 32), lane_at(v, 48)));
 }
 
-// Sums relative to a maximum: s = sum 2^((x - m) c), t = sum (..)(x - m) c.
+// Sums relative to a maximum (-inf: none): s = sum 2^((x - m) c), t = sum of
+// that times (x - m) c.
 struct Sums {
   float m, s, t;
 };
 template <bool kEnt>
 __device__ __forceinline__ Sums fold_sums(Sums a, float c) {
-  const float m = fold64(a.m, Max{});
-  const float d = (a.m - m) * c;
-  const float f = exp2_(d);
   Sums r;
-  r.m = m;
+  r.m = fold64(a.m, Max{});
+  const float d = (a.m - (r.m == neg_inf() ? 0.0f : r.m)) * c;
+  const float f = exp2_(d);
   r.s = fold64(a.s * f, Add{});
   r.t = kEnt ? fold64(f * fmaf(a.s, fmaxf(d, kFloor), a.t), Add{}) : 0.0f;
   return r;
@@ -336,6 +354,39 @@ __device__ __forceinline__ uint64_t fold64_max(uint64_t v) {
   }
   return v;
 }
+// The largest of one value a lane below which fewer than k of 64 lanes (k <= 8:
+// of 16 groups of 4, for a quarter of the work) lie above it: `top`'s bound.
+__device__ __forceinline__ float kth_value(float v, int k) {
+  int rank = 0;
+  if (k <= 8) {
+    float q = v;
+    q = fmaxf(q, __shfl_xor(q, 16));
+    q = fmaxf(q, __shfl_xor(q, 32));
+    const auto above = [&](float o) { rank += o > q ? 1 : 0; };
+    above(dpp<0x121>(q));
+    above(dpp<0x122>(q));
+    above(dpp<0x123>(q));
+    above(dpp<0x124>(q));
+    above(dpp<0x125>(q));
+    above(dpp<0x126>(q));
+    above(dpp<0x127>(q));
+    above(dpp<0x128>(q));
+    above(dpp<0x129>(q));
+    above(dpp<0x12A>(q));
+    above(dpp<0x12B>(q));
+    above(dpp<0x12C>(q));
+    above(dpp<0x12D>(q));
+    above(dpp<0x12E>(q));
+    above(dpp<0x12F>(q));
+    v = q;
+  } else {
+#pragma unroll 8
+    for (int j = 0; j < 64; ++j) rank += lane_at(v, j) > v ? 1 : 0;
+  }
+  // of the values with fewer than k above them, the least
+  return -fold64(rank < k ? -v : neg_inf(), Max{});
+}
+
 // The k-th largest (k >= 1) of one key a lane.
 __device__ __forceinline__ uint64_t kth64(uint64_t key, int k) {
   const int lane = threadIdx.x & 63;
@@ -356,7 +407,8 @@ __device__ __forceinline__ uint64_t kth64(uint64_t key, int k) {
 
 struct TopLds {
   uint64_t group[64];  // largest key of lane i of every wave
-  uint64_t limit;
+  float bound;         // what the top-th largest is not below,
+  int cut;             // and, at the bound, where the last needed one's chunk ends
   uint32_t count;
   uint64_t cand[kCandidates];
 };
@@ -405,18 +457,37 @@ __device__ __forceinline__ void table_add(const Table& t, int32_t id, float w, f
   }
 }
 
-// p_i (f0 + f1 ln p_i) of a logit.
+// p_i (f0 + f1 log2 p_i) of a logit x, as e (g0 + g1 d) with d = x c - R in one
+// operation, e = 2^d and R = m c rounded: what the rounding leaves out and l are
+// in g0 and g1.  A wild row takes d = (x - m) c.
 struct Dense {
-  float m, l, c, f0, f1;
+  float c, ref, m, g0, g1;
+  bool plain;  // neither wild nor with a factor that is not finite
+  __device__ __forceinline__ Dense(float m_, float l, float c_, float f0, float f1)
+      : c(c_), ref(m_ * c_), m(m_) {
+    const bool wild = !(fabsf(ref) <= kWild);
+    const float k = (wild ? 0.0f : fmaf(-m, c, ref)) - l;
+    const float f = exp2_(k);
+    g0 = fmaf(f1, k, f0) * f;
+    g1 = f1 * f;
+    const float inf = __builtin_huge_valf();
+    plain = !wild && fabsf(g0) < inf && fabsf(g1) < inf;
+  }
+  template <bool kLog>
+  __device__ __forceinline__ float scaled(float d) const {
+    const float e = exp2_(d);
+    return kLog ? e * fmaf(g1, fmaxf(d, kFloor), g0) : e * g0;
+  }
+  // plain rows
   template <bool kLog>
   __device__ __forceinline__ float at(float x) const {
-    const float d = fmaf(x - m, c, -l);
-    const float p = exp2_(d);
-    return kLog ? p * fmaf(f1, fmaxf(d, kFloor), f0) : p * f0;
+    return scaled<kLog>(fmaf(x, c, -ref));
   }
-  // A factor that is not finite must not reach the excluded actions.
-  __device__ __forceinline__ bool odd() const {
-    return !(fabsf(f0) < __builtin_huge_valf()) || !(fabsf(f1) < __builtin_huge_valf()) || l != l;
+  // any row: an excluded action's is 0 whatever the factors
+  template <bool kLog>
+  __device__ __forceinline__ float any(float x) const {
+    if (x == neg_inf()) return 0.0f;
+    return scaled<kLog>(fabsf(ref) <= kWild ? fmaf(x, c, -ref) : (x - m) * c);
   }
 };
 
@@ -460,20 +531,23 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
   // before a chunk's own start is dropped when it is used.
   int me = tid;  // (renewed for each pass)
   auto load = [&](int t, const T* x, const uint8_t* legal, int last) {
-    const int oc = min((t * bd + me) * kE, last);
-    raw[t] = load_at<T, u32x4>(x + oc);
+    // (an unsigned byte offset to a uniform base: no 64-bit address arithmetic)
+    const uint32_t oc = min((t * bd + me) * kE, last);
+    const uint32_t bytes = oc * static_cast<uint32_t>(sizeof(T));
+    raw[t] = load_at<T, u32x4>(
+        reinterpret_cast<const T*>(reinterpret_cast<const char*>(x) + bytes));
     if constexpr (kMask) mk[t] = load_at<uint8_t, Word>(legal + oc);
   };
   // The chunk's values, excluded ones -inf; true where it holds any.
-  auto values = [&](int t, float (&x)[kE]) {
+  auto values = [&](int t, float (&x)[kE], int ln) {
     unpack<T>(raw[t], x);
     if constexpr (kMask) {
 #pragma unroll
       for (int j = 0; j < kE; ++j)
         if (((mk[t] >> (8 * j)) & 0xFF) == 0) x[j] = neg_inf();
     }
-    if ((t + 1) * bd * kE > len) {
-      const int o = (t * bd + me) * kE, oc = min(o, len - kE);
+    if ((t + 1) * bd * kE > ln) {
+      const int o = (t * bd + me) * kE, oc = min(o, ln - kE);
 #pragma unroll
       for (int j = 0; j < kE; ++j)
         if (oc + j < o) x[j] = neg_inf();
@@ -482,10 +556,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     if constexpr (kSums && kSecond && kMask) raw[t] = pack<T>(x);
   };
   // The same again, once values() has left the exclusions in the registers.
-  auto again = [&](int t, float (&x)[kE]) {
+  auto again = [&](int t, float (&x)[kE], int ln) {
     renew(raw[t]);
     if constexpr (kSums) unpack<T>(raw[t], x);
-    else values(t, x);
+    else values(t, x, ln);
   };
 
   int64_t r = blockIdx.x;
@@ -552,42 +626,74 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     }
 
     // -- the sums --
-    Sums u{kLowest, 0.0f, 0.0f};
-    int best_o = 0;  // start of the first chunk with the lane's maximum
+    // A lane's reference R is its largest x c so far, never below -kWild (what
+    // is, adds nothing unless the whole row is: that one is wild, below).
+    // Then d = x c - R is one operation an element and the sums are rescaled
+    // once a chunk.
+    Sums u{neg_inf(), 0.0f, 0.0f};
+    float ref = -kWild;
+    int best_o = 0;                       // start of the first chunk with the lane's maximum
+    float chunk_max[kTop ? kN : 1];
     if constexpr (kSums) {
+      const int ln = renewed_scalar(len);
       renew(me);
 #pragma unroll
       for (int t = 0; t < kN; ++t) {
-        if (t * bd * kE < len) {
+        if constexpr (kTop) chunk_max[t] = neg_inf();
+        if (t * bd * kE < ln) {
           float x[kE];
-          values(t, x);
-          float cm = x[0];
-#pragma unroll
-          for (int j = 1; j < kE; ++j) cm = fmaxf(cm, x[j]);
-          if constexpr (kTop) best_o = cm > u.m ? (t * bd + me) * kE : best_o;
-          const float m = fmaxf(u.m, cm);
-          const float dm = (u.m - m) * a.c;
-          const float f = exp2_(dm);
-          if constexpr (kEnt) u.t = f * fmaf(u.s, fmaxf(dm, kFloor), u.t);
-          u.m = m;
-          float s = 0.0f;
+          values(t, x, ln);
+          const float cm = largest<kE>(x);
+          if constexpr (kTop) {
+            best_o = cm > u.m ? (t * bd + me) * kE : best_o;
+            chunk_max[t] = cm;
+          }
+          u.m = fmaxf(u.m, cm);
+          const float to = fmaxf(cm * a.c, ref);
+          const float step = ref - to;
+          const float f = exp2_(step);
+          ref = to;
+          float s = 0.0f, tc = 0.0f;
 #pragma unroll
           for (int j = 0; j < kE; ++j) {
-            const float d = (x[j] - m) * a.c;
+            const float d = fmaf(x[j], a.c, -to);
             const float e = exp2_(d);
             s += e;
-            if constexpr (kEnt) u.t = fmaf(e, fmaxf(d, kFloor), u.t);
+            if constexpr (kEnt) tc = fmaf(e, kMask ? fmaxf(d, kFloor) : d, tc);
           }
+          if constexpr (kEnt && !kMask) {
+            // 0 * -inf: an excluded action (rare without a mask: not worth the
+            // clamp on every element)
+            if (__any(tc != tc)) {
+              tc = 0.0f;
+#pragma unroll
+              for (int j = 0; j < kE; ++j) {
+                const float d = fmaf(x[j], a.c, -to);
+                tc = fmaf(exp2_(d), fmaxf(d, kFloor), tc);
+              }
+            }
+          }
+          if constexpr (kEnt) u.t = fmaf(f, fmaf(u.s, step, u.t), tc);
           u.s = fmaf(u.s, f, s);
         }
         if constexpr (!kSecond) load(t, nx, nl, nlast);
       }
     }
 
+    // from R to the lane's exact m c
+    if constexpr (kSums) {
+      if (ref > -kWild) {
+        const float off = fmaf(u.m, a.c, -ref);
+        const float f = exp2_(-off);
+        if constexpr (kEnt) u.t = f * fmaf(-off, u.s, u.t);
+        u.s *= f;
+      }
+    }
+
     // -- across the lanes and waves --
     uint64_t lane_key = 0;
     if constexpr (kTop) {
-      if (u.s > 0.0f) lane_key = top_key(u.m, static_cast<uint32_t>(lo + best_o));
+      if (u.m > neg_inf()) lane_key = top_key(u.m, static_cast<uint32_t>(lo + best_o));
       if (nw > 1 && lane_key != 0)
         atomicMax(reinterpret_cast<unsigned long long*>(&top_lds.group[lane]),
                   static_cast<unsigned long long>(lane_key));
@@ -612,7 +718,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
       const float* const q = red[par][lane & (kMaxWaves - 1)];
       const bool in = lane < nw;
       if constexpr (kSums) {
-        u = in ? Sums{q[0], q[1], q[2]} : Sums{kLowest, 0.0f, 0.0f};
+        u = in ? Sums{q[0], q[1], q[2]} : Sums{neg_inf(), 0.0f, 0.0f};
         u = fold_sums<kEnt>(u, a.c);
       }
       if constexpr (kTarget) {
@@ -624,7 +730,32 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     }
     float m, l;
     if constexpr (kSums) {
-      m = u.s == 0.0f ? 0.0f : u.m;
+      if (u.m > neg_inf() && !(fabsf(u.m * a.c) <= kWild)) {
+        // a wild row: once more, from memory
+        u.s = u.t = 0.0f;
+        for (int i = tid; i < len; i += bd) {
+          const float d = (logit<T>(a, r, lo + i) - u.m) * a.c;
+          const float e = exp2_(d);
+          u.s += e;
+          if constexpr (kEnt) u.t = fmaf(e, fmaxf(d, kFloor), u.t);
+        }
+        u.s = fold64(u.s, Add{});
+        u.t = fold64(u.t, Add{});
+        if (nw > 1) {
+          __syncthreads();
+          if (lane == 0) {
+            red[par][wave][1] = u.s;
+            red[par][wave][2] = u.t;
+          }
+          __syncthreads();
+          u.s = u.t = 0.0f;
+          for (int w = 0; w < nw; ++w) {
+            u.s += red[par][w][1];
+            u.t += red[par][w][2];
+          }
+        }
+      }
+      m = u.m == neg_inf() ? 0.0f : u.m;
       l = u.s == 0.0f ? 0.0f : log2f(u.s);
     } else {
       m = g.stats[2 * r];
@@ -660,30 +791,47 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
         // without the bound costs a pass over the row for each of `top`.)
         if (wave == 0) {
           const uint64_t key = nw == 1 ? lane_key : top_lds.group[lane];
-          const uint64_t lim = kth64(key, g.top);
+          const float v = key == 0 ? neg_inf() : key_value(key);
+          const int at = key == 0 ? 0x7FFFFFFF : static_cast<int>(key_index(key));
+          const float tv = kth_value(v, g.top);
+          // of those at the bound, as many as `top` still needs, the first
+          const uint64_t tied = __ballot(v == tv && key != 0);
+          const int need = g.top - __builtin_popcountll(__ballot(v > tv));
+          int cut = -kE;
+          if (tied != 0 && need > 0) {
+            const int mine = v == tv ? at : 0x7FFFFFFF;
+            int rank = 0;
+            if (tied & (tied - 1)) {
+              for (int j = 0; j < 64; ++j) rank += __builtin_amdgcn_readlane(mine, j) < mine ? 1 : 0;
+            }
+            const uint64_t in = tied & __ballot(rank < need);
+            // the last of them: the one with the largest start
+            int far = (in >> lane & 1) != 0 ? mine : -1;
+            for (int o = 32; o > 0; o >>= 1) far = max(far, __shfl_xor(far, o));
+            cut = far;
+          }
           top_lds.group[lane] = 0;
           if (lane == 0) {
-            top_lds.limit = lim;
+            top_lds.bound = tv;
+            top_lds.cut = cut + kE;
             top_lds.count = 0;
           }
         }
         __syncthreads();
-        const uint64_t lim = top_lds.limit;
         const bool odd = l != l;
-        const float tv = lim == 0 ? neg_inf() : key_value(lim);
-        const int ti = lim == 0 ? 0 : static_cast<int>(key_index(lim)) - lo + kE;
+        const float tv = top_lds.bound;
+        const int ti = top_lds.cut - lo;
+        const int ln = renewed_scalar(len);
         renew(me);
 #pragma unroll
         for (int t = 0; t < kN; ++t) {
-          if (t * bd * kE < len && !odd) {
-            float x[kE];
-            again(t, x);
-            float cm = x[0];
-#pragma unroll
-            for (int j = 1; j < kE; ++j) cm = fmaxf(cm, x[j]);
+          if (t * bd * kE < ln && !odd) {
+            const float cm = chunk_max[t];
             const int o = (t * bd + me) * kE;
-            if (cm > tv || (cm == tv && o < ti)) {
-              const int oc = min(o, len - kE);
+            if (cm > tv || (cm == tv && o < ti && tv > neg_inf())) {
+              float x[kE];
+              again(t, x, ln);
+              const int oc = min(o, ln - kE);
 #pragma unroll
               for (int j = 0; j < kE; ++j)
                 if (x[j] > tv || (x[j] == tv && oc + j < ti)) {
@@ -840,24 +988,26 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     if constexpr (kGrad) {
       const Dense dn{m, l, a.c, f0, f1};
       constexpr bool kLog = kOp == kLogprobsGrad;
-      const bool odd = dn.odd();
       T* const gb = static_cast<T*>(g.grad) + r * g.grad_ld + lo;
+      const int ln = renewed_scalar(len);
       renew(me);
 #pragma unroll
       for (int t = 0; t < kN; ++t) {
-        if (t * bd * kE < len) {
+        if (t * bd * kE < ln) {
           float x[kE], y[kE];
-          again(t, x);
-          const int o = (t * bd + me) * kE, oc = min(o, len - kE);
+          again(t, x, ln);
+          const int o = (t * bd + me) * kE, oc = min(o, ln - kE);
+          if (dn.plain) {
 #pragma unroll
-          for (int j = 0; j < kE; ++j) y[j] = dn.template at<kLog>(x[j]);
-          if (odd) {
+            for (int j = 0; j < kE; ++j) y[j] = dn.template at<kLog>(x[j]);
+          } else {
 #pragma unroll
-            for (int j = 0; j < kE; ++j) y[j] = x[j] == neg_inf() ? 0.0f : y[j];
+            for (int j = 0; j < kE; ++j) y[j] = dn.template any<kLog>(x[j]);
           }
-          if (o + kE <= len) {
-            store_at<T>(gb + o, pack<T>(y));
-          } else if (o < len) {
+          if (o + kE <= ln) {
+            const uint32_t bytes = static_cast<uint32_t>(o) * static_cast<uint32_t>(sizeof(T));
+            store_at<T>(reinterpret_cast<T*>(reinterpret_cast<char*>(gb) + bytes), pack<T>(y));
+          } else if (o < ln) {
 #pragma unroll
             for (int j = 0; j < kE; ++j)
               if (oc + j >= o) gb[oc + j] = static_cast<T>(y[j]);
@@ -868,7 +1018,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
       // the listed actions once more, with their weights (a barrier: after the
       // dense stores of whichever wave)
       const auto fix = [&](int id, float w, float x) {
-        gb[id - lo] = static_cast<T>(dn.template at<kLog>(x) + w);
+        gb[id - lo] = static_cast<T>(dn.template any<kLog>(x) + w);
       };
       if constexpr (kTarget) {
         __syncthreads();
@@ -922,39 +1072,6 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
 }
 
 // ---- rows of up to four chunks a lane: a wave each ----
-
-// The largest of one value a lane below which fewer than k of 64 lanes (k <= 8:
-// of 16 groups of 4, for a quarter of the work) lie above it: `top`'s bound.
-__device__ __forceinline__ float kth_value(float v, int k) {
-  int rank = 0;
-  if (k <= 8) {
-    float q = v;
-    q = fmaxf(q, __shfl_xor(q, 16));
-    q = fmaxf(q, __shfl_xor(q, 32));
-    const auto above = [&](float o) { rank += o > q ? 1 : 0; };
-    above(dpp<0x121>(q));
-    above(dpp<0x122>(q));
-    above(dpp<0x123>(q));
-    above(dpp<0x124>(q));
-    above(dpp<0x125>(q));
-    above(dpp<0x126>(q));
-    above(dpp<0x127>(q));
-    above(dpp<0x128>(q));
-    above(dpp<0x129>(q));
-    above(dpp<0x12A>(q));
-    above(dpp<0x12B>(q));
-    above(dpp<0x12C>(q));
-    above(dpp<0x12D>(q));
-    above(dpp<0x12E>(q));
-    above(dpp<0x12F>(q));
-    v = q;
-  } else {
-#pragma unroll 8
-    for (int j = 0; j < 64; ++j) rank += lane_at(v, j) > v ? 1 : 0;
-  }
-  // of the values with fewer than k above them, the least
-  return -fold64(rank < k ? -v : neg_inf(), Max{});
-}
 
 // kC chunks a lane, the values in registers as floats; the next row's chunks
 // are under way while a row is worked on.  No barrier is needed: what goes
@@ -1054,17 +1171,29 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       for (int i = 0; i < kX; ++i) lane_max = fmaxf(lane_max, x[i]);
       m = fold64(lane_max, Max{});
       if (m == neg_inf()) m = 0.0f;  // empty, or only NaN
-      float s = 0.0f, u = 0.0f;
+      float s = 0.0f, u = 0.0f, off = 0.0f;
+      const float ref = m * a.c;
+      if (fabsf(ref) <= kWild) {
+        off = fmaf(m, a.c, -ref);
 #pragma unroll
-      for (int i = 0; i < kX; ++i) {
-        const float d = (x[i] - m) * a.c;
-        const float e = exp2_(d);
-        s += e;
-        if constexpr (kLp) u = fmaf(e, fmaxf(d, kFloor), u);
+        for (int i = 0; i < kX; ++i) {
+          const float d = fmaf(x[i], a.c, -ref);
+          const float e = exp2_(d);
+          s += e;
+          if constexpr (kLp) u = fmaf(e, fmaxf(d, kFloor), u);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kX; ++i) {
+          const float d = (x[i] - m) * a.c;
+          const float e = exp2_(d);
+          s += e;
+          if constexpr (kLp) u = fmaf(e, fmaxf(d, kFloor), u);
+        }
       }
       s = fold64(s, Add{});
-      l = s == 0.0f ? 0.0f : log2f(s);
-      if constexpr (kLp) mean = s == 0.0f ? 0.0f : fold64(u, Add{}) / s;
+      l = s == 0.0f ? 0.0f : log2f(s) - off;
+      if constexpr (kLp) mean = s == 0.0f ? 0.0f : fold64(u, Add{}) / s - off;
     } else {
       m = g.stats[2 * r];
       l = g.stats[2 * r + 1];
@@ -1139,7 +1268,7 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
     }
 
     // -- the listed entries --
-    Dense dn{m, l, a.c, 0.0f, 0.0f};
+    float f0 = 0.0f, f1 = 0.0f;
     const auto clear = [&] {
 #pragma unroll
       for (int t = 0; t < kX / 4; ++t)
@@ -1189,7 +1318,7 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       float scale = 0.0f, ce = 0.0f, h = 0.0f;
       if constexpr (kGrad) {
         scale = (g.weight != nullptr ? g.weight[r * g.weight_stride] : 1.0f) * a.inv_t;
-        dn.f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
+        f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
       }
       float ew[kGrad ? kHeld : 1];  // the weights, until the values are read
 #pragma unroll
@@ -1276,34 +1405,41 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
         fence();
         const bool clash = __ballot(ti >= 0 && tag[slot(static_cast<int>(ti))] != lane) != 0;
         fence();
-        if (ti >= 0) row[slot(static_cast<int>(ti))] = clash ? 0.0f : gt * a.inv_t;
+        const bool on = ti >= 0 && logit<T>(a, r, ti) > neg_inf();
+        if (ti >= 0) row[slot(static_cast<int>(ti))] = clash || !on ? 0.0f : gt * a.inv_t;
         fence();
         if (clash && lane == 0)
           for (int j = 0; j < g.top; ++j) {
             const int64_t id = g.top_action[r * g.top + j];
-            if (id >= 0 && id < a.v) row[slot(static_cast<int>(id))] += g.gt[r * g.top + j] * a.inv_t;
+            if (id >= 0 && id < a.v && logit<T>(a, r, id) > neg_inf())
+              row[slot(static_cast<int>(id))] += g.gt[r * g.top + j] * a.inv_t;
           }
         fence();
       }
-      if (lane == 0 && in) row[slot(static_cast<int>(given))] += gl * a.inv_t;
+      if (lane == 0 && in && given_x > neg_inf()) row[slot(static_cast<int>(given))] += gl * a.inv_t;
       fence();
       const float gh = g.gh != nullptr ? g.gh[r * g.ghs] : 0.0f;
-      dn.f0 = -(sum + (gh != 0.0f ? gh * g.entropy[r] : 0.0f)) * a.inv_t;
-      dn.f1 = -gh * kLn2 * a.inv_t;
+      f0 = -(sum + (gh != 0.0f ? gh * g.entropy[r] : 0.0f)) * a.inv_t;
+      f1 = -gh * kLn2 * a.inv_t;
     }
 
     // -- the gradient --
     if constexpr (kGrad) {
+      constexpr bool kLog = kOp == kLogprobsGrad;
+      const Dense dn{m, l, a.c, f0, f1};
       T* const gb = static_cast<T*>(g.grad) + r * g.grad_ld;
       renew(me);
 #pragma unroll
       for (int t = 0; t < kC; ++t) {
         float y[kE];
 #pragma unroll
-        for (int j = 0; j < kE; ++j) {
-          const float v = x[t * kE + j];
-          y[j] = dn.template at<kOp == kLogprobsGrad>(v) + row[(t * 64 + me) * kE + j];
-          if (v == neg_inf()) y[j] = 0.0f;
+        for (int j = 0; j < kE; ++j) y[j] = row[(t * 64 + me) * kE + j];
+        if (dn.plain) {
+#pragma unroll
+          for (int j = 0; j < kE; ++j) y[j] += dn.template at<kLog>(x[t * kE + j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kE; ++j) y[j] += dn.template any<kLog>(x[t * kE + j]);
         }
         const int o = (t * 64 + me) * kE;
         if (t < kC / 2 || o + kE <= a.v) {
@@ -1333,10 +1469,10 @@ __global__ __launch_bounds__(kJoin) void k_join(Rows a, JoinArgs g) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x;
   const PartSums* const ps = g.lp.sums + r * g.parts;
-  Sums u{kLowest, 0.0f, 0.0f};
+  Sums u{neg_inf(), 0.0f, 0.0f};
   if (lane < g.parts) u = Sums{ps[lane].m, ps[lane].s, ps[lane].t};
   u = fold_sums<!kLoss>(u, a.c);
-  const float m = u.s == 0.0f ? 0.0f : u.m;
+  const float m = u.m == neg_inf() ? 0.0f : u.m;
   const float l = u.s == 0.0f ? 0.0f : log2f(u.s);
   float* const stats = kLoss ? g.ds.stats : g.lp.stats;
   if (tid == 0 && stats != nullptr) {
@@ -1524,7 +1660,7 @@ __global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
         }
       }
     }
-    Dense dn{m, l, a.c, 0.0f, 0.0f};
+    float f0 = 0.0f, f1 = 0.0f;
     if constexpr (kGrad) {
 #pragma unroll
       for (int e = 0; e < kEach; ++e) dq[l16 + 16 * e] = 0.0f;
@@ -1593,7 +1729,7 @@ __global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
             if (e.id >= 0 && e.id < a.v)
               dq[e.id] -= scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
           }
-        dn.f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
+        f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
         __syncthreads();
       }
     }
@@ -1614,17 +1750,18 @@ __global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
       }
       sum = __shfl(sum, tid & 48);  // the row's first lane's
       const float gh = g.gh != nullptr ? g.gh[r * g.ghs] : 0.0f;
-      dn.f0 = -(sum + (gh != 0.0f ? gh * g.entropy[r] : 0.0f)) * a.inv_t;
-      dn.f1 = -gh * kLn2 * a.inv_t;
+      f0 = -(sum + (gh != 0.0f ? gh * g.entropy[r] : 0.0f)) * a.inv_t;
+      f1 = -gh * kLn2 * a.inv_t;
       __syncthreads();
     }
     if constexpr (kGrad) {
+      const Dense dn{m, l, a.c, f0, f1};
       T* const gb = static_cast<T*>(g.grad) + r * g.grad_ld;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
         const int i = l16 + 16 * e;
         if (i < a.v && live) {
-          const float y = dn.template at<kOp == kLogprobsGrad>(x[e]) + dq[i];
+          const float y = dn.template any<kOp == kLogprobsGrad>(x[e]) + dq[i];
           gb[i] = static_cast<T>(x[e] == neg_inf() ? 0.0f : y);
         }
       }
