@@ -47,9 +47,10 @@ constexpr int kTinyMax = 64;       // rows of up to this many actions: 16 lanes 
 constexpr int kMaxWaves = 16;
 constexpr int kMaxSplit = 64;      // parts of a row
 constexpr int kCandidates = 512;   // top actions: LDS list
+constexpr int kWaveCandidates = 256;  // of a wave alone (a multiple of 64)
 constexpr int kFewChunks = 4;      // chunks a lane in the kernels for short rows
-constexpr int kChunks = 16;        // for long ones
-constexpr int kMaskChunks = 8;     // with a mask
+constexpr int kMidChunks = 8;      // for longer ones; the most with a mask
+constexpr int kChunks = 16;        // the most without
 
 struct Rows {
   const void* x;
@@ -354,37 +355,27 @@ __device__ __forceinline__ uint64_t fold64_max(uint64_t v) {
   }
   return v;
 }
-// The largest of one value a lane below which fewer than k of 64 lanes (k <= 8:
-// of 16 groups of 4, for a quarter of the work) lie above it: `top`'s bound.
-__device__ __forceinline__ float kth_value(float v, int k) {
-  int rank = 0;
-  if (k <= 8) {
-    float q = v;
-    q = fmaxf(q, __shfl_xor(q, 16));
-    q = fmaxf(q, __shfl_xor(q, 32));
-    const auto above = [&](float o) { rank += o > q ? 1 : 0; };
-    above(dpp<0x121>(q));
-    above(dpp<0x122>(q));
-    above(dpp<0x123>(q));
-    above(dpp<0x124>(q));
-    above(dpp<0x125>(q));
-    above(dpp<0x126>(q));
-    above(dpp<0x127>(q));
-    above(dpp<0x128>(q));
-    above(dpp<0x129>(q));
-    above(dpp<0x12A>(q));
-    above(dpp<0x12B>(q));
-    above(dpp<0x12C>(q));
-    above(dpp<0x12D>(q));
-    above(dpp<0x12E>(q));
-    above(dpp<0x12F>(q));
-    v = q;
-  } else {
-#pragma unroll 8
-    for (int j = 0; j < 64; ++j) rank += lane_at(v, j) > v ? 1 : 0;
+// One of the lanes' values with at least k of them at or above it, and usually
+// few more (-inf where fewer than k lanes hold any): a bound of the k-th largest
+// element from below.  Bisection between the least and the largest, counting
+// with ballots on the scalar unit: six steps or so, where ranking every lane
+// against every other takes 192 vector operations.
+__device__ __forceinline__ float kth_bound(float v, int k) {
+  const float inf = __builtin_huge_valf();
+  const bool any = v > neg_inf();
+  if (__builtin_popcountll(__ballot(any)) < k) return neg_inf();
+  float lo = -fold64(any ? -v : -inf, Max{});
+  float hi = fold64(v, Max{});
+  const int enough = k + (k >> 3) + 1;
+  for (int step = 0; step < 24; ++step) {
+    const float mid = fmaf(lo, 0.5f, hi * 0.5f);
+    if (!(mid > lo && mid < hi)) break;
+    const int n = __builtin_popcountll(__ballot(v >= mid));
+    if (n >= k) lo = mid;
+    else hi = mid;
+    if (n >= k && n <= enough) break;
   }
-  // of the values with fewer than k above them, the least
-  return -fold64(rank < k ? -v : neg_inf(), Max{});
+  return -fold64(v >= lo ? -v : -inf, Max{});
 }
 
 // The k-th largest (k >= 1) of one key a lane.
@@ -405,11 +396,16 @@ __device__ __forceinline__ uint64_t kth64(uint64_t key, int k) {
          static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(lo), src));
 }
 
+struct Found {
+  float x;
+  int i;
+};
 struct TopLds {
   uint64_t group[64];  // largest key of lane i of every wave
   float bound;         // what the top-th largest is not below,
   int cut;             // and, at the bound, where the last needed one's chunk ends
-  uint32_t count;
+  uint32_t chunks, count;
+  int chunk[kCandidates];  // starts of the chunks that reach the bound
   uint64_t cand[kCandidates];
 };
 
@@ -508,7 +504,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
   constexpr bool kTop = kOp == kLogprobsTop;
   constexpr bool kEnt = kOp == kLogprobs || kOp == kLogprobsTop;
   constexpr bool kTarget = kOp == kDistill || kOp == kDistillFused || kOp == kDistillGrad;
-  constexpr bool kSecond = kTop || kGrad;            // a second pass over the registers
+  constexpr bool kSecond = kGrad;                    // a second pass over the registers
   constexpr int kHeld = kN == kFewChunks ? 4 : 1;    // target entries a lane keeps
   using Word = std::conditional_t<kE == 8, uint64_t, uint32_t>;  // a chunk's mask bytes
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
@@ -633,7 +629,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     Sums u{neg_inf(), 0.0f, 0.0f};
     float ref = -kWild;
     int best_o = 0;                       // start of the first chunk with the lane's maximum
-    float chunk_max[kTop ? kN : 1];
+    float chunk_max[kTop ? kN : 1];       // (NaN: see largest())
     if constexpr (kSums) {
       const int ln = renewed_scalar(len);
       renew(me);
@@ -644,7 +640,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
           float x[kE];
           values(t, x, ln);
           const float cm = largest<kE>(x);
-          if constexpr (kTop) {
+          if constexpr (kTop) {  // (chunks past the row's end hold -inf)
             best_o = cm > u.m ? (t * bd + me) * kE : best_o;
             chunk_max[t] = cm;
           }
@@ -793,7 +789,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
           const uint64_t key = nw == 1 ? lane_key : top_lds.group[lane];
           const float v = key == 0 ? neg_inf() : key_value(key);
           const int at = key == 0 ? 0x7FFFFFFF : static_cast<int>(key_index(key));
-          const float tv = kth_value(v, g.top);
+          const float tv = kth_bound(v, g.top);
           // of those at the bound, as many as `top` still needs, the first
           const uint64_t tied = __ballot(v == tv && key != 0);
           const int need = g.top - __builtin_popcountll(__ballot(v > tv));
@@ -815,6 +811,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
             top_lds.bound = tv;
             top_lds.cut = cut + kE;
             top_lds.count = 0;
+            top_lds.chunks = 0;
           }
         }
         __syncthreads();
@@ -823,28 +820,29 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
         const int ti = top_lds.cut - lo;
         const int ln = renewed_scalar(len);
         renew(me);
+        // The chunks that hold them are few: listed, and read once more (their
+        // registers have gone to the next row already), an element a lane.
 #pragma unroll
         for (int t = 0; t < kN; ++t) {
-          if (t * bd * kE < ln && !odd) {
-            const float cm = chunk_max[t];
-            const int o = (t * bd + me) * kE;
-            if (cm > tv || (cm == tv && o < ti && tv > neg_inf())) {
-              float x[kE];
-              again(t, x, ln);
-              const int oc = min(o, ln - kE);
-#pragma unroll
-              for (int j = 0; j < kE; ++j)
-                if (x[j] > tv || (x[j] == tv && oc + j < ti)) {
-                  const uint32_t at = atomicAdd(&top_lds.count, 1u);
-                  if (at < kCandidates)
-                    top_lds.cand[at] = top_key(x[j], static_cast<uint32_t>(lo + oc + j));
-                }
-            }
+          const float cm = chunk_max[t];
+          const int o = (t * bd + me) * kE;
+          if (!odd && (cm > tv || (cm == tv && o < ti && tv > neg_inf()))) {
+            const uint32_t at = atomicAdd(&top_lds.chunks, 1u);
+            if (at < kCandidates) top_lds.chunk[at] = o;
           }
-          load(t, nx, nl, nlast);
         }
         __syncthreads();
-        const int found = odd ? 0 : static_cast<int>(top_lds.count);
+        const int listed = static_cast<int>(top_lds.chunks);
+        for (int i = tid; i < min(listed, kCandidates) * kE; i += bd) {
+          const int o = top_lds.chunk[i / kE], e = min(o, ln - kE) + i % kE;
+          const float x = logit<T>(a, r, lo + e);
+          if (e >= o && (x > tv || (x == tv && e < ti))) {
+            const uint32_t at = atomicAdd(&top_lds.count, 1u);
+            if (at < kCandidates) top_lds.cand[at] = top_key(x, static_cast<uint32_t>(lo + e));
+          }
+        }
+        __syncthreads();
+        const int found = odd ? 0 : listed > kCandidates ? listed : static_cast<int>(top_lds.count);
         const auto put = [&](int rank, uint64_t key) {
           if (g.part_keys != nullptr) {
             g.part_keys[part * g.top + rank] = key;
@@ -1023,18 +1021,23 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
       if constexpr (kTarget) {
         __syncthreads();
         if (twice[par] != 0) {
-          __syncthreads();
+          // the entries in order, through the other row's table (at rest)
+          unsigned char* const base = dyn + static_cast<size_t>(par ^ 1) * g.hash * 12;
+          int32_t* const lid = reinterpret_cast<int32_t*>(base);
+          float* const lw = reinterpret_cast<float*>(base + static_cast<size_t>(g.hash) * 4);
+          float* const lx = reinterpret_cast<float*>(base + static_cast<size_t>(g.hash) * 8);
           table_clear(tab, tid, bd);
+          for (int j = tid; j < g.t.k; j += bd) {
+            const Entry e = target_entry(g.t, r, j);
+            const bool in = e.id >= lo && e.id < lo + len;
+            lid[j] = in ? static_cast<int32_t>(e.id) : -1;
+            lx[j] = in ? logit<T>(a, r, e.id) : neg_inf();
+            lw[j] = -scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
+          }
           __syncthreads();
           if (tid == 0)
-            for (int j = 0; j < g.t.k; ++j) {
-              const Entry e = target_entry(g.t, r, j);
-              if (e.id < lo || e.id >= lo + len) continue;
-              const float x = logit<T>(a, r, e.id);
-              if (x > neg_inf())
-                table_add(tab, static_cast<int>(e.id),
-                          -scale * (target_mass(g.t, a.c, e.z, mass.z) * inv), x);
-            }
+            for (int j = 0; j < g.t.k; ++j)
+              if (lid[j] >= 0 && lx[j] > neg_inf()) table_add(tab, lid[j], lw[j], lx[j]);
           __syncthreads();
         }
         for (int i = tid; i <= tab.mask; i += bd)
@@ -1089,7 +1092,8 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
   // The row's values, then its listed weights: chunk (t, lane) at
   // (t * 64 + lane) * kE, the row's last actions where their chunk has them.
   __shared__ __attribute__((aligned(16))) float row[kTarget || kGrad ? 64 * kX : 1];
-  __shared__ uint64_t cand[kOp == kLogprobsTop ? 64 : 1];
+  __shared__ Found cand[kOp == kLogprobsTop ? kWaveCandidates : 1];
+  __shared__ uint64_t keys[kOp == kLogprobsTop ? kWaveCandidates : 1];
   const int lane = threadIdx.x;
   const int last = a.v - kE;
   const auto fence = [] { __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront"); };
@@ -1221,30 +1225,44 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
         g.top_logprob[r * g.top + rank] =
             odd ? l : key == 0 ? neg_inf() : log_p(a, key_value(key), m, l);
       };
-      const float bound = fmaxf(kth_value(lane_max, g.top), kLowest);
+      const float bound = fmaxf(kth_bound(lane_max, g.top), kLowest);
       int found = 0;
       renew(me);
       if (!odd) {
 #pragma unroll
-        for (int i = 0; i < kX; ++i) {
-          const uint64_t hit = __ballot(x[i] >= bound);
-          if (hit != 0) {
-            const int at = found + __builtin_amdgcn_mbcnt_hi(
-                static_cast<uint32_t>(hit >> 32),
-                __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hit), 0));
-            const int o = (i / kE * 64 + me) * kE;
-            if (x[i] >= bound && at < 64)
-              cand[at] = top_key(x[i], static_cast<uint32_t>(min(o, last) + i % kE));
-            found += __builtin_popcountll(hit);
+        for (int t = 0; t < kC; ++t) {
+          const int oc = min((t * 64 + me) * kE, last);
+#pragma unroll
+          for (int j = 0; j < kE; ++j) {
+            const bool in = x[t * kE + j] >= bound;
+            const uint64_t hit = __ballot(in);
+            if (hit != 0) {
+              const int at = __builtin_amdgcn_mbcnt_hi(
+                  static_cast<uint32_t>(hit >> 32),
+                  __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hit), found));
+              if (in && at < kWaveCandidates) cand[at] = Found{x[t * kE + j], oc + j};
+              found += __builtin_popcountll(hit);
+            }
           }
         }
       }
-      if (found <= 64) {
+      if (found <= kWaveCandidates) {
         fence();
-        const uint64_t key = lane < found ? cand[lane] : 0;
-        int rank = 0;
-        for (int j = 0; j < found; ++j) rank += cand[j] > key ? 1 : 0;
-        if (lane < found && rank < g.top) put(rank, key);
+        const int whole = (found + 63) & ~63;
+        for (int i = lane; i < whole; i += 64) {
+          const Found f = cand[i];  // (past `found`: not used)
+          keys[i] = i < found ? top_key(f.x, static_cast<uint32_t>(f.i)) : 0;
+        }
+        fence();
+        for (int i = lane; i < whole; i += 64) {
+          const uint64_t key = keys[i];
+          int rank = 0;
+          for (int j = 0; j < found; j += 8) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) rank += keys[j + q] > key ? 1 : 0;
+          }
+          if (i < found && rank < g.top) put(rank, key);
+        }
         if (lane >= found && lane < g.top) put(lane, 0);
         fence();
       } else {
@@ -1375,8 +1393,16 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
             if (id >= 0 && logit<T>(a, r, id) > neg_inf())
               row[slot(id)] = -scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
           }
-        } else if (lane == 0) {  // in list order
-          for (int j = 0; j < k; ++j) {
+        } else {  // in list order
+#pragma unroll
+          for (int i = 0; i < kHeld; ++i) {
+            for (int q = 0; q < 64 && q + i * 64 < k; ++q) {
+              const int id = __builtin_amdgcn_readlane(eid[i], q);
+              const float w = lane_at(ew[i], q);
+              if (id >= 0 && lane == 0) row[slot(id)] += w;
+            }
+          }
+          for (int j = kHeld * 64; j < k && lane == 0; ++j) {
             const Entry e = target_entry(g.t, r, j);
             const int id = entry_id(e);
             if (id >= 0 && logit<T>(a, r, id) > neg_inf())
@@ -1778,7 +1804,7 @@ struct Launch {
   dim3 grid;
   int waves;       // 0: k_tiny; 1 with `wave` chunks: k_wave
   int wave;        // chunks a lane of k_wave (1, 2 or 4), 0: k_rows
-  bool few;        // kFewChunks chunks a lane
+  int chunks;      // a lane of k_rows
   unsigned lds;    // dynamic, bytes
   hipStream_t stream;
 };

@@ -26,7 +26,7 @@ static_assert(OS_AZ_NO_WORKSPACE_ACTIONS * 4 <= 4 * kWaveFew);
 struct Plan {
   int waves;  // 0: k_tiny
   int wave;   // chunks a lane of k_wave, 0: k_rows
-  bool few;
+  int chunks;  // a lane of k_rows
   Parts pt;
   dim3 grid;
 };
@@ -57,7 +57,6 @@ bool short_rows(const Rows& a, int size, Plan* p) {
   const int64_t bytes = int64_t{a.v} * size;
   if (bytes > kWaveFew && a.v > kTinyMax) return false;
   p->pt = Parts{1, a.v};
-  p->few = true;
   if (a.v <= kTinyMax) {
     p->grid = dim3(static_cast<unsigned>(std::min<int64_t>(up(a.n, kTinyRows), kCus * 8)));
     return true;
@@ -68,27 +67,30 @@ bool short_rows(const Rows& a, int size, Plan* p) {
   return true;
 }
 
-int64_t wave_bytes(const Rows& a) { return (a.legal ? kMaskChunks : kChunks) * kKib; }
+int64_t wave_bytes(const Rows& a) { return (a.legal ? kMidChunks : kChunks) * kKib; }
+
+// Chunks a lane and waves for `bytes` a workgroup: with `wide` as many waves
+// as four chunks each allow (few rows: each is over sooner), else as few as the
+// registers allow (more rows at once, fewer waves to join).
+void fit(const Rows& a, int64_t bytes, bool wide, Plan* p) {
+  const int64_t most = wave_bytes(a);
+  if (wide && bytes <= kMaxWaves * kWaveFew) p->chunks = kFewChunks;
+  else if (bytes <= kMidChunks * kKib || most == kMidChunks * kKib) p->chunks = kMidChunks;
+  else p->chunks = kChunks;
+  p->waves = static_cast<int>(up(bytes, p->chunks * kKib));
+}
 
 // Kernels that need the row's sums.
 Plan sums_plan(const Rows& a, int size) {
   Plan p{};
   if (short_rows(a, size, &p)) return p;
-  const int64_t bytes = int64_t{a.v} * size, wave = wave_bytes(a);
-  int64_t parts = 1;
-  if (bytes <= 4 * kWaveFew) {
-    p.few = true;
-  } else if (a.n < 2 * kCus) {
-    parts = std::max(up(bytes, kMaxWaves * wave), std::min(up(2 * kCus, a.n), bytes / (16 * kKib)));
-    parts = std::min<int64_t>(parts, kMaxSplit);
-  } else {
-    parts = up(bytes, kMaxWaves * wave);
-  }
-  p.pt = split(a.v, parts);
-  const int64_t each = int64_t{p.pt.part} * size;
-  if (each <= 4 * kWaveFew) p.few = true;
-  p.waves = static_cast<int>(up(each, p.few ? kWaveFew : wave));
-  p.grid = row_grid(a.n, p, p.few ? 24 : 16);
+  const int64_t bytes = int64_t{a.v} * size, most = kMaxWaves * wave_bytes(a);
+  int64_t parts = up(bytes, most);
+  if (a.n < 2 * kCus && bytes > 4 * kWaveFew)
+    parts = std::max(parts, std::min(up(2 * kCus, a.n), bytes / (16 * kKib)));
+  p.pt = split(a.v, std::min<int64_t>(parts, kMaxSplit));
+  fit(a, int64_t{p.pt.part} * size, a.n * p.pt.parts < 4 * kCus, &p);
+  p.grid = row_grid(a.n, p, p.chunks == kChunks ? 16 : p.chunks == kMidChunks ? 20 : 28);
   return p;
 }
 
@@ -97,9 +99,8 @@ Plan grad_plan(const Rows& a, int size) {
   Plan p{};
   if (short_rows(a, size, &p)) return p;
   const int64_t bytes = int64_t{a.v} * size;
-  p.few = bytes <= 4 * kWaveFew;
   p.pt = split(a.v, up(bytes, 64 * kKib));
-  p.waves = static_cast<int>(up(int64_t{p.pt.part} * size, p.few ? kWaveFew : wave_bytes(a)));
+  fit(a, int64_t{p.pt.part} * size, a.n * p.pt.parts < 4 * kCus, &p);
   p.grid = row_grid(a.n, p, 16);
   return p;
 }
@@ -107,7 +108,7 @@ Plan grad_plan(const Rows& a, int size) {
 int type_size(int dtype) { return dtype == OS_AZ_F32 ? 4 : 2; }
 
 Launch launch(const Rows& a, const Plan& p, void* stream) {
-  return Launch{a, p.pt, p.grid, p.waves, p.wave, p.few, 0, static_cast<hipStream_t>(stream)};
+  return Launch{a, p.pt, p.grid, p.waves, p.wave, p.chunks, 0, static_cast<hipStream_t>(stream)};
 }
 
 // Each part's sums and top keys, and the rows' stats where a caller wants none.

@@ -27,16 +27,20 @@ void launch_rows(const Launch& c, const G& g) {
     return;
   }
   const dim3 block(64 * c.waves);
+  const auto go = [&](auto mask, auto chunks) {
+    hipLaunchKernelGGL((k_rows<T, decltype(mask)::value, decltype(chunks)::value, kOp>), c.grid,
+                       block, c.lds, c.stream, c.a, c.pt, g);
+  };
+  constexpr std::integral_constant<int, kFewChunks> few;
+  constexpr std::integral_constant<int, kMidChunks> mid;
+  constexpr std::integral_constant<int, kChunks> many;
   if (c.a.legal != nullptr) {
-    if (c.few)
-      hipLaunchKernelGGL((k_rows<T, true, kFewChunks, kOp>), c.grid, block, c.lds, c.stream, c.a, c.pt, g);
-    else
-      hipLaunchKernelGGL((k_rows<T, true, kMaskChunks, kOp>), c.grid, block, c.lds, c.stream, c.a, c.pt, g);
+    if (c.chunks == few) go(std::true_type{}, few);
+    else go(std::true_type{}, mid);
   } else {
-    if (c.few)
-      hipLaunchKernelGGL((k_rows<T, false, kFewChunks, kOp>), c.grid, block, c.lds, c.stream, c.a, c.pt, g);
-    else
-      hipLaunchKernelGGL((k_rows<T, false, kChunks, kOp>), c.grid, block, c.lds, c.stream, c.a, c.pt, g);
+    if (c.chunks == few) go(std::false_type{}, few);
+    else if (c.chunks == mid) go(std::false_type{}, mid);
+    else go(std::false_type{}, many);
   }
 }
 
