@@ -167,6 +167,15 @@ __device__ __forceinline__ void store_at(T* p, W w) {
   reinterpret_cast<P*>(p)->w = w;
 }
 
+// A chunk's mask bytes.
+template <int kE>
+struct __attribute__((packed, aligned(1))) MaskWord {
+  uint32_t w[kE / 4];
+  __device__ __forceinline__ bool allows(int j) const {
+    return (w[j / 4] & (0xFFu << (8 * (j % 4)))) != 0;
+  }
+};
+
 template <class T>
 __device__ __forceinline__ void unpack(u32x4 r, float (&x)[kPer<T>]) {
   if constexpr (std::is_same_v<T, float>) {
@@ -206,6 +215,18 @@ __device__ __forceinline__ u32x4 pack(const float (&x)[kPer<T>]) {
   return r;
 }
 
+// A load at a uniform address of memory that the kernel does not write: on the
+// scalar unit, in a queue of its own (vector loads come back in order, so one
+// for a single value would wait for the whole next row's).
+template <class V>
+__device__ __forceinline__ V uniform(const V* p, int64_t i) {
+  return reinterpret_cast<const __attribute__((address_space(4))) V*>(
+      reinterpret_cast<uintptr_t>(p))[i];
+}
+__device__ __forceinline__ int64_t uniform_id(const void* p, int wide, int64_t i) {
+  return wide ? uniform(static_cast<const int64_t*>(p), i)
+              : uniform(static_cast<const int32_t*>(p), i);
+}
 __device__ __forceinline__ int64_t get_id(const void* p, int wide, int64_t i) {
   return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
 }
@@ -264,11 +285,35 @@ __device__ __forceinline__ T fold16(T v, F f) {
 __device__ __forceinline__ float lane_at(float v, int i) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
 }
-template <class F>
-__device__ __forceinline__ float fold64(float v, F f) {
-  v = fold16(v, f);
-  return f(f(lane_at(v, 0), lane_at(v, 16)), f(lane_at(v, 32), lane_at(v, 48)));
+// Over the wave: within rows of 16 lanes as above, then row 0 into 1 and 2 into
+// 3, then both into the last row; a uniform result.  Written out because the
+// compiler quiets both operands of every maximum (three instructions a step for
+// one).  A DPP operand needs two wait states after its write: the s_nop.
+#define OSP_FOLD64(op)                                                    \
+  "s_nop 1\n"                                                             \
+  op " %0, %1, %1 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n"       \
+  "s_nop 1\n"                                                             \
+  op " %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n"       \
+  "s_nop 1\n"                                                             \
+  op " %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n"           \
+  "s_nop 1\n"                                                             \
+  op " %0, %0, %0 row_mirror row_mask:0xf bank_mask:0xf\n"                \
+  "s_nop 1\n"                                                             \
+  op " %0, %0, %0 row_bcast:15 row_mask:0xa bank_mask:0xf\n"              \
+  "s_nop 1\n"                                                             \
+  op " %0, %0, %0 row_bcast:31 row_mask:0xc bank_mask:0xf\n"              \
+  "s_nop 1\n"
+__device__ __forceinline__ float fold64(float v, Max) {
+  float r;
+  asm volatile(OSP_FOLD64("v_max_f32_dpp") : "=&v"(r) : "v"(v));
+  return lane_at(r, 63);
 }
+__device__ __forceinline__ float fold64(float v, Add) {
+  float r;
+  asm volatile(OSP_FOLD64("v_add_f32_dpp") : "=&v"(r) : "v"(v));
+  return lane_at(r, 63);
+}
+#undef OSP_FOLD64
 
 // Sums relative to a maximum (-inf: none): s = sum 2^((x - m) c), t = sum of
 // that times (x - m) c.
@@ -313,6 +358,58 @@ __device__ __forceinline__ Entry target_entry(const Target& t, int64_t r, int j)
   e.id = t.ids != nullptr ? get_id(t.ids, t.wide, r * t.ids_ld + j) : j;
   e.z = e.id < 0 ? neg_inf() : target_value(t, r * t.val_ld + j);
   return e;
+}
+// Entries first, first + step, .. of a row (those below k; the others none):
+// every load is issued before one is waited for.  id -1: none or past the
+// actions (then bad); z: the value, -inf where there is no mass.
+template <int kCount>
+__device__ __forceinline__ void target_entries(const Target& t, int64_t r, int first, int step,
+                                               int v, int (&id)[kCount], float (&z)[kCount],
+                                               float& bad) {
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) {
+    id[i] = -1;
+    z[i] = neg_inf();
+  }
+  if (t.k == 0) return;
+  // (uniform: how many of the batches hold any entry)
+  const int rounds = min(kCount, (t.k + step - 1) / step);
+  const auto at = [&](int i) { return min(first + i * step, t.k - 1); };
+  const auto all = [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i)
+      if (i < rounds) f(i);
+  };
+  int64_t raw[kCount];
+  if (t.ids == nullptr) {
+    all([&](int i) { raw[i] = at(i); });
+  } else if (t.wide) {
+    const int64_t* const p = static_cast<const int64_t*>(t.ids) + r * t.ids_ld;
+    all([&](int i) { raw[i] = p[at(i)]; });
+  } else {
+    const int32_t* const p = static_cast<const int32_t*>(t.ids) + r * t.ids_ld;
+    all([&](int i) { raw[i] = p[at(i)]; });
+  }
+  const auto values = [&](auto* p) {
+    p += r * t.val_ld;
+    all([&](int i) { z[i] = static_cast<float>(p[at(i)]); });
+  };
+  switch (t.type) {
+    case OS_AZ_LOGITS_F32:
+    case OS_AZ_WEIGHTS_F32: values(static_cast<const float*>(t.val)); break;
+    case OS_AZ_LOGITS_BF16: values(static_cast<const __bf16*>(t.val)); break;
+    case OS_AZ_LOGITS_F16: values(static_cast<const _Float16*>(t.val)); break;
+    default: values(static_cast<const int32_t*>(t.val)); break;
+  }
+  all([&](int i) {
+    // (selects only: written with && and an if, the compiler of ROCm 7.2 lost the
+    // weights' z <= 0 case)
+    const bool in = (first + i * step < t.k) & (raw[i] >= 0), past = raw[i] >= v;
+    const bool none = !in | ((t.type >= OS_AZ_WEIGHTS_F32) & (z[i] <= 0.0f));
+    bad = in & past ? 1.0f : bad;
+    id[i] = in & !past ? static_cast<int>(raw[i]) : -1;
+    z[i] = none ? neg_inf() : z[i];
+  });
 }
 // Running (maximum, mass relative to it) of target entries.
 struct Mass {
@@ -366,7 +463,7 @@ __device__ __forceinline__ float kth_bound(float v, int k) {
   if (__builtin_popcountll(__ballot(any)) < k) return neg_inf();
   float lo = -fold64(any ? -v : -inf, Max{});
   float hi = fold64(v, Max{});
-  const int enough = k + (k >> 3) + 1;
+  const int enough = k + (k >> 2) + 3;
   for (int step = 0; step < 24; ++step) {
     const float mid = fmaf(lo, 0.5f, hi * 0.5f);
     if (!(mid > lo && mid < hi)) break;
@@ -506,7 +603,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
   constexpr bool kTarget = kOp == kDistill || kOp == kDistillFused || kOp == kDistillGrad;
   constexpr bool kSecond = kGrad;                    // a second pass over the registers
   constexpr int kHeld = kN == kFewChunks ? 4 : 1;    // target entries a lane keeps
-  using Word = std::conditional_t<kE == 8, uint64_t, uint32_t>;  // a chunk's mask bytes
+  using Word = MaskWord<kE>;
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   __shared__ float red[2][kMaxWaves][8];
   __shared__ float red2[2][kMaxWaves][2];
@@ -540,7 +637,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     if constexpr (kMask) {
 #pragma unroll
       for (int j = 0; j < kE; ++j)
-        if (((mk[t] >> (8 * j)) & 0xFF) == 0) x[j] = neg_inf();
+        if (!mk[t].allows(j)) x[j] = neg_inf();
     }
     if ((t + 1) * bd * kE > ln) {
       const int o = (t * bd + me) * kE, oc = min(o, ln - kE);
@@ -587,26 +684,17 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     Table tab{};
     if constexpr (kTarget) {
       const int k = g.t.k;
-      const auto take = [&](Entry e) {
-        if (e.id >= a.v) bad = 1.0f;
-        mass_add(g.t, a.c, e.z, mass);
-      };
+      target_entries<kHeld>(g.t, r, tid, bd, a.v, eid, ez, bad);
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) {
-        eid[i] = -1;
-        ez[i] = neg_inf();
         ex[i] = neg_inf();
-        if (i * bd < k) {
-          const int j = tid + i * bd;
-          if (j < k) {
-            const Entry e = target_entry(g.t, r, j);
-            take(e);
-            eid[i] = e.id < 0 || e.id >= a.v ? -1 : static_cast<int>(e.id);
-            ez[i] = e.z;
-          }
-        }
+        mass_add(g.t, a.c, ez[i], mass);
       }
-      for (int j = tid + kHeld * bd; j < k; j += bd) take(target_entry(g.t, r, j));
+      for (int j = tid + kHeld * bd; j < k; j += bd) {
+        const Entry e = target_entry(g.t, r, j);
+        if (e.id >= a.v) bad = 1.0f;
+        mass_add(g.t, a.c, e.z, mass);
+      }
 #pragma unroll
       for (int i = 0; i < kHeld; ++i)
         if (i * bd < k && eid[i] >= 0) ex[i] = logit<T>(a, r, eid[i]);
@@ -619,6 +707,14 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
         table_clear(tab, tid, bd);
         if (tid == 0) twice[par] = 0;
       }
+    }
+
+    // -- the given action's logit --
+    int64_t given = -1;
+    float given_x = neg_inf();
+    if constexpr (kEnt || kOp == kLogprobsGrad) {
+      if (g.actions != nullptr) given = uniform_id(g.actions, g.wide, r);
+      if (given >= 0 && given < a.v) given_x = logit<T>(a, r, given);
     }
 
     // -- the sums --
@@ -754,8 +850,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
       m = u.m == neg_inf() ? 0.0f : u.m;
       l = u.s == 0.0f ? 0.0f : log2f(u.s);
     } else {
-      m = g.stats[2 * r];
-      l = g.stats[2 * r + 1];
+      m = uniform(g.stats, 2 * r);
+      l = uniform(g.stats, 2 * r + 1);
     }
 
     // -- log probabilities --
@@ -771,10 +867,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
             g.stats[2 * r + 1] = l;
           }
           if (g.actions != nullptr) {
-            const int64_t id = get_id(g.actions, g.wide, r);
-            g.logprob[r] = id < 0 ? 0.0f
-                           : id >= a.v ? __builtin_nanf("")
-                                       : log_p(a, logit<T>(a, r, id), m, l);
+            g.logprob[r] = given < 0 ? 0.0f
+                           : given >= a.v ? __builtin_nanf("")
+                                          : log_p(a, given_x, m, l);
           }
         }
       }
@@ -888,7 +983,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     if constexpr (kTarget) {
       inv = mass.s == 0.0f ? 0.0f : 1.0f / mass.s;
       if constexpr (kGrad) {
-        scale = (g.weight != nullptr ? g.weight[r * g.weight_stride] : 1.0f) * a.inv_t;
+        scale = (g.weight != nullptr ? uniform(g.weight, r * g.weight_stride) : 1.0f) * a.inv_t;
         f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
       }
       float ce = 0.0f, h = 0.0f;
@@ -947,14 +1042,14 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     int act = -1;
     float act_w = 0.0f, act_x = neg_inf();
     if constexpr (kOp == kLogprobsGrad) {
-      const int64_t id = g.actions != nullptr && g.gl != nullptr ? get_id(g.actions, g.wide, r) : -1;
-      float sum = id >= a.v ? __builtin_nanf("") : 0.0f;
-      if (id >= 0 && id < a.v) {
-        act = static_cast<int>(id);
-        act_w = g.gl[r * g.gls];
-        sum = act_w;
-        act_w *= a.inv_t;
-        act_x = logit<T>(a, r, id);
+      float sum = 0.0f;
+      if (g.gl != nullptr && given >= 0) {
+        sum = given >= a.v ? __builtin_nanf("") : uniform(g.gl, r * g.gls);
+        if (given < a.v) {
+          act = static_cast<int>(given);
+          act_w = sum * a.inv_t;
+          act_x = given_x;
+        }
       }
       if (g.top > 0) {
         int64_t ti = -1;
@@ -977,8 +1072,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
           if (x > neg_inf() && !table_put(tab, static_cast<int>(ti), gt * a.inv_t, x)) twice[par] = 1;
         }
       }
-      const float gh = g.gh != nullptr ? g.gh[r * g.ghs] : 0.0f;
-      f0 = -(sum + (gh != 0.0f ? gh * g.entropy[r] : 0.0f)) * a.inv_t;
+      const float gh = g.gh != nullptr ? uniform(g.gh, r * g.ghs) : 0.0f;
+      f0 = -(sum + (gh != 0.0f ? gh * uniform(g.entropy, r) : 0.0f)) * a.inv_t;
       f1 = -gh * kLn2 * a.inv_t;
     }
 
@@ -1088,7 +1183,7 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
   constexpr bool kLp = kOp == kLogprobs || kOp == kLogprobsTop;
   constexpr bool kTarget = kOp == kDistill || kOp == kDistillFused || kOp == kDistillGrad;
   constexpr int kHeld = 8;  // target entries a lane keeps in registers
-  using Word = std::conditional_t<kE == 8, uint64_t, uint32_t>;
+  using Word = MaskWord<kE>;
   // The row's values, then its listed weights: chunk (t, lane) at
   // (t * 64 + lane) * kE, the row's last actions where their chunk has them.
   __shared__ __attribute__((aligned(16))) float row[kTarget || kGrad ? 64 * kX : 1];
@@ -1115,6 +1210,11 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
   const int edge = a.v / kE * kE, shift = (kE - a.v % kE) % kE;
   const auto slot = [&](int id) { return id + (id >= edge ? shift : 0); };
 
+  // How many elements of a chunk come before its own start (see load()).
+  int drop[kC - kC / 2];
+#pragma unroll
+  for (int t = kC / 2; t < kC; ++t) drop[t - kC / 2] = (t * 64 + lane) * kE - min((t * 64 + lane) * kE, last);
+
   load(blockIdx.x);
   for (int64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
     // -- the row's values --
@@ -1130,20 +1230,19 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       if constexpr (kMask) {
 #pragma unroll
         for (int j = 0; j < kE; ++j)
-          if (((mk[t] >> (8 * j)) & 0xFF) == 0) x[t * kE + j] = neg_inf();
+          if (!mk[t].allows(j)) x[t * kE + j] = neg_inf();
       }
       if (t >= kC / 2) {  // (the first half is full: fewer chunks would do else)
-        const int o = (t * 64 + me) * kE, drop = o - min(o, last);
 #pragma unroll
         for (int j = 0; j < kE; ++j)
-          if (j < drop) x[t * kE + j] = neg_inf();
+          if (j < drop[t - kC / 2]) x[t * kE + j] = neg_inf();
       }
     }
     // -- what else the row needs from memory, ahead of the next row's loads --
     int64_t given = -1;
     float given_x = neg_inf();
     if constexpr (kLp || kOp == kLogprobsGrad) {
-      if (g.actions != nullptr) given = get_id(g.actions, g.wide, r);
+      if (g.actions != nullptr) given = uniform_id(g.actions, g.wide, r);
       if (given >= 0 && given < a.v) given_x = logit<T>(a, r, given);
     }
     int eid[kTarget ? kHeld : 1];
@@ -1154,17 +1253,7 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       return e.id < 0 || e.id >= a.v ? -1 : static_cast<int>(e.id);
     };
     if constexpr (kTarget) {
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        eid[i] = -1;
-        ez[i] = neg_inf();
-        if (i * 64 < g.t.k && lane + i * 64 < g.t.k) {
-          const Entry e = target_entry(g.t, r, lane + i * 64);
-          if (e.id >= a.v) bad = 1.0f;
-          eid[i] = entry_id(e);
-          ez[i] = e.z;
-        }
-      }
+      target_entries<kHeld>(g.t, r, lane, 64, a.v, eid, ez, bad);
     }
     if (r + gridDim.x < a.n) load(r + gridDim.x);
 
@@ -1199,8 +1288,8 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       l = s == 0.0f ? 0.0f : log2f(s) - off;
       if constexpr (kLp) mean = s == 0.0f ? 0.0f : fold64(u, Add{}) / s - off;
     } else {
-      m = g.stats[2 * r];
-      l = g.stats[2 * r + 1];
+      m = uniform(g.stats, 2 * r);
+      l = uniform(g.stats, 2 * r + 1);
     }
 
     if constexpr (kLp) {
@@ -1335,7 +1424,7 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       const float inv = mass.s == 0.0f ? 0.0f : 1.0f / mass.s;
       float scale = 0.0f, ce = 0.0f, h = 0.0f;
       if constexpr (kGrad) {
-        scale = (g.weight != nullptr ? g.weight[r * g.weight_stride] : 1.0f) * a.inv_t;
+        scale = (g.weight != nullptr ? uniform(g.weight, r * g.weight_stride) : 1.0f) * a.inv_t;
         f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
       }
       float ew[kGrad ? kHeld : 1];  // the weights, until the values are read
@@ -1414,7 +1503,7 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
     }
     if constexpr (kOp == kLogprobsGrad) {
       const bool in = g.gl != nullptr && given >= 0 && given < a.v;
-      const float gl = in ? g.gl[r * g.gls] : 0.0f;
+      const float gl = in ? uniform(g.gl, r * g.gls) : 0.0f;
       float sum = g.gl != nullptr && given >= a.v ? __builtin_nanf("") : gl;
       clear();
       fence();
@@ -1444,8 +1533,8 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       }
       if (lane == 0 && in && given_x > neg_inf()) row[slot(static_cast<int>(given))] += gl * a.inv_t;
       fence();
-      const float gh = g.gh != nullptr ? g.gh[r * g.ghs] : 0.0f;
-      f0 = -(sum + (gh != 0.0f ? gh * g.entropy[r] : 0.0f)) * a.inv_t;
+      const float gh = g.gh != nullptr ? uniform(g.gh, r * g.ghs) : 0.0f;
+      f0 = -(sum + (gh != 0.0f ? gh * uniform(g.entropy, r) : 0.0f)) * a.inv_t;
       f1 = -gh * kLn2 * a.inv_t;
     }
 

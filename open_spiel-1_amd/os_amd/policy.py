@@ -315,6 +315,16 @@ def _new_distill(logits, target, target_actions, legal, kind, temperature, keep_
   return loss, entropy, stats
 
 
+def _once(backward):
+  """torch.autograd.function.once_differentiable, but for the usual call (no
+  graph of the gradient is asked for), which needs none of its bookkeeping."""
+  checked = torch.autograd.function.once_differentiable(backward)
+
+  def call(ctx, *grads):
+    return (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
+  return call
+
+
 class _LogProbs(torch.autograd.Function):
 
   @staticmethod
@@ -329,7 +339,7 @@ class _LogProbs(torch.autograd.Function):
     return logprob, entropy, top_action, top_logprob
 
   @staticmethod
-  @torch.autograd.function.once_differentiable
+  @_once
   def backward(ctx, g_logprob, g_entropy, _, g_top):
     if g_logprob is None and g_entropy is None and g_top is None:
       return (None,) * 5
@@ -360,7 +370,7 @@ class _Distill(torch.autograd.Function):
     return loss, entropy
 
   @staticmethod
-  @torch.autograd.function.once_differentiable
+  @_once
   def backward(ctx, g_loss, _):
     if g_loss is None:
       return (None,) * 6
