@@ -331,8 +331,31 @@ __device__ __forceinline__ Sums fold_sums(Sums a, float c) {
   return r;
 }
 
-// A target's unnormalised value (weights: those not above 0 are no mass, -inf)
-// and its mass relative to the row's largest.
+// A target's unnormalised mass is relative to a reference, the row's largest
+// value: logits 2^((z - ref) c), weights z times the power of two that brings
+// the reference near 1 (sums neither overflow nor vanish, and no division an
+// entry).  An entry without mass has the value 0 (weights) or -inf (logits).
+__device__ __forceinline__ bool is_weights(const Target& t) { return t.type >= OS_AZ_WEIGHTS_F32; }
+__device__ __forceinline__ float no_mass(const Target& t) { return is_weights(t) ? 0.0f : neg_inf(); }
+__device__ __forceinline__ int weight_scale_bits(float ref) {
+  return max(0x7E800000 - (__float_as_int(ref) & 0x7F800000), 0x00800000);
+}
+__device__ __forceinline__ float target_mass(const Target& t, float c, float z, float ref) {
+  if (is_weights(t)) return z * __int_as_float(weight_scale_bits(ref));
+  return exp2_((z - (ref == neg_inf() ? 0.0f : ref)) * c);
+}
+// What takes a mass relative to `from` to one relative to `to`, not below it.
+__device__ __forceinline__ float mass_step(const Target& t, float c, float from, float to) {
+  if (is_weights(t)) {
+    const int b = 0x3F800000 + weight_scale_bits(to) - weight_scale_bits(from);
+    return b <= 0 ? 0.0f : __int_as_float(b);
+  }
+  return from == to ? 1.0f : exp2_((from - to) * c);
+}
+// ln q of a mass share.
+__device__ __forceinline__ float log_share(float q) {
+  return kLn2 * fmaxf(__builtin_amdgcn_logf(q), kFloor);
+}
 __device__ __forceinline__ float target_value(const Target& t, int64_t i) {
   float z;
   switch (t.type) {
@@ -342,11 +365,7 @@ __device__ __forceinline__ float target_value(const Target& t, int64_t i) {
     case OS_AZ_WEIGHTS_F32: z = static_cast<const float*>(t.val)[i]; break;
     default: z = static_cast<float>(static_cast<const int32_t*>(t.val)[i]); break;
   }
-  return z <= 0.0f ? neg_inf() : z;
-}
-__device__ __forceinline__ float target_mass(const Target& t, float c, float z, float ref) {
-  if (z == neg_inf()) return 0.0f;
-  return t.type >= OS_AZ_WEIGHTS_F32 ? z / ref : exp2f((z - ref) * c);
+  return z <= 0.0f ? 0.0f : z;
 }
 // Entry j of a row: its action (< 0: none) and value.
 struct Entry {
@@ -356,7 +375,7 @@ struct Entry {
 __device__ __forceinline__ Entry target_entry(const Target& t, int64_t r, int j) {
   Entry e;
   e.id = t.ids != nullptr ? get_id(t.ids, t.wide, r * t.ids_ld + j) : j;
-  e.z = e.id < 0 ? neg_inf() : target_value(t, r * t.val_ld + j);
+  e.z = e.id < 0 ? no_mass(t) : target_value(t, r * t.val_ld + j);
   return e;
 }
 // Entries first, first + step, .. of a row (those below k; the others none):
@@ -369,7 +388,7 @@ __device__ __forceinline__ void target_entries(const Target& t, int64_t r, int f
 #pragma unroll
   for (int i = 0; i < kCount; ++i) {
     id[i] = -1;
-    z[i] = neg_inf();
+    z[i] = no_mass(t);
   }
   if (t.k == 0) return;
   // (uniform: how many of the batches hold any entry)
@@ -380,12 +399,16 @@ __device__ __forceinline__ void target_entries(const Target& t, int64_t r, int f
     for (int i = 0; i < kCount; ++i)
       if (i < rounds) f(i);
   };
-  int64_t raw[kCount];
+  int raw[kCount];  // (of an int64 only whether it is below 0 or past the actions counts)
   if (t.ids == nullptr) {
     all([&](int i) { raw[i] = at(i); });
   } else if (t.wide) {
     const int64_t* const p = static_cast<const int64_t*>(t.ids) + r * t.ids_ld;
-    all([&](int i) { raw[i] = p[at(i)]; });
+    int64_t wide[kCount];
+    all([&](int i) { wide[i] = p[at(i)]; });
+    all([&](int i) {
+      raw[i] = static_cast<int>(wide[i] < 0 ? -1 : wide[i] < v ? wide[i] : int64_t{v});
+    });
   } else {
     const int32_t* const p = static_cast<const int32_t*>(t.ids) + r * t.ids_ld;
     all([&](int i) { raw[i] = p[at(i)]; });
@@ -405,10 +428,10 @@ __device__ __forceinline__ void target_entries(const Target& t, int64_t r, int f
     // (selects only: written with && and an if, the compiler of ROCm 7.2 lost the
     // weights' z <= 0 case)
     const bool in = (first + i * step < t.k) & (raw[i] >= 0), past = raw[i] >= v;
-    const bool none = !in | ((t.type >= OS_AZ_WEIGHTS_F32) & (z[i] <= 0.0f));
+    const bool none = !in | (is_weights(t) & (z[i] <= 0.0f));
     bad = in & past ? 1.0f : bad;
-    id[i] = in & !past ? static_cast<int>(raw[i]) : -1;
-    z[i] = none ? neg_inf() : z[i];
+    id[i] = in & !past ? raw[i] : -1;
+    z[i] = none ? no_mass(t) : z[i];
   });
 }
 // Running (maximum, mass relative to it) of target entries.
@@ -416,17 +439,23 @@ struct Mass {
   float z, s;
 };
 __device__ __forceinline__ void mass_add(const Target& t, float c, float z, Mass& a) {
-  if (z > a.z) {
-    a.s = a.s * target_mass(t, c, a.z, z) + 1.0f;
-    a.z = z;
-  } else if (z != neg_inf()) {
-    a.s += target_mass(t, c, z, a.z);
-  }
+  const float to = fmaxf(a.z, z);
+  a.s = fmaf(a.s, mass_step(t, c, a.z, to), target_mass(t, c, z, to));
+  a.z = to;
+}
+template <int kCount>
+__device__ __forceinline__ Mass mass_of(const Target& t, float c, const float (&z)[kCount]) {
+  Mass a{z[0], 0.0f};
+#pragma unroll
+  for (int i = 1; i < kCount; ++i) a.z = fmaxf(a.z, z[i]);
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) a.s += target_mass(t, c, z[i], a.z);
+  return a;
 }
 template <class MaxF, class AddF>
 __device__ __forceinline__ Mass mass_fold(const Target& t, float c, Mass a, MaxF maxf, AddF addf) {
   const float z = maxf(a.z);
-  return Mass{z, addf(a.s * target_mass(t, c, a.z, z))};
+  return Mass{z, addf(a.s * mass_step(t, c, a.z, z))};
 }
 
 // ---- top actions ----
@@ -686,10 +715,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
       const int k = g.t.k;
       target_entries<kHeld>(g.t, r, tid, bd, a.v, eid, ez, bad);
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        ex[i] = neg_inf();
-        mass_add(g.t, a.c, ez[i], mass);
-      }
+      for (int i = 0; i < kHeld; ++i) ex[i] = neg_inf();
+      mass = mass_of(g.t, a.c, ez);
       for (int j = tid + kHeld * bd; j < k; j += bd) {
         const Entry e = target_entry(g.t, r, j);
         if (e.id >= a.v) bad = 1.0f;
@@ -814,7 +841,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
         u = fold_sums<kEnt>(u, a.c);
       }
       if constexpr (kTarget) {
-        mass = in ? Mass{q[3], q[4]} : Mass{neg_inf(), 0.0f};
+        mass = in ? Mass{q[3], q[4]} : Mass{no_mass(g.t), 0.0f};
         mass = mass_fold(g.t, a.c, mass, [](float z) { return fold64(z, Max{}); },
                          [](float z) { return fold64(z, Add{}); });
         bad = fold64(in ? q[5] : 0.0f, Max{});
@@ -992,7 +1019,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
         if constexpr (kOp != kDistillGrad) {
           if (q != 0.0f) {
             if (id >= 0) ce -= q * log_p(a, x, m, l);
-            h -= q * (kLn2 * log2f(q));
+            h -= q * log_share(q);
           }
         }
         if constexpr (kGrad) {
@@ -1397,8 +1424,10 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       for (int j = lane + kHeld * 64; j < k; j += 64)
         if (target_entry(g.t, r, j).id >= a.v) bad = 1.0f;
       bool clash = false;
+      mass = mass_of(g.t, a.c, ez);
+      for (int j = lane + kHeld * 64; j < k; j += 64)
+        mass_add(g.t, a.c, target_entry(g.t, r, j).z, mass);
       each([&](int id, float z, int j) {
-        mass_add(g.t, a.c, z, mass);
         if (kGrad && g.t.ids != nullptr && id >= 0) tag[slot(id)] = j;
       });
       if constexpr (kGrad) {
@@ -1436,7 +1465,7 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
           if constexpr (kOp != kDistillGrad) {
             if (q != 0.0f) {
               if (eid[i] >= 0) ce -= q * log_p(a, xi, m, l);
-              h -= q * (kLn2 * log2f(q));
+              h -= q * log_share(q);
             }
           }
           if constexpr (kGrad) {
@@ -1452,7 +1481,7 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
         if constexpr (kOp != kDistillGrad) {
           if (q != 0.0f) {
             if (id >= 0) ce -= q * log_p(a, row[slot(id)], m, l);
-            h -= q * (kLn2 * log2f(q));
+            h -= q * log_share(q);
           }
         }
       }
@@ -1637,7 +1666,7 @@ __global__ __launch_bounds__(kJoin) void k_join(Rows a, JoinArgs g) {
     for (int i = found + tid; i < q.top; i += kJoin) put(i, 0);
   } else {
     const DistillArgs& q = g.ds;
-    Mass mass{neg_inf(), 0.0f};
+    Mass mass{no_mass(q.t), 0.0f};
     float bad = 0.0f;
     for (int j = tid; j < q.t.k; j += kJoin) {
       const Entry e = target_entry(q.t, r, j);
@@ -1656,7 +1685,7 @@ __global__ __launch_bounds__(kJoin) void k_join(Rows a, JoinArgs g) {
     __syncthreads();
     const bool in = lane < kJoin / 64;
     const float* const w0 = red[lane & (kJoin / 64 - 1)];
-    mass = in ? Mass{w0[0], w0[1]} : Mass{neg_inf(), 0.0f};
+    mass = in ? Mass{w0[0], w0[1]} : Mass{no_mass(q.t), 0.0f};
     bad = fold64(in ? w0[2] : 0.0f, Max{});
     mass = mass_fold(q.t, a.c, mass, maxf, addf);
     const float inv = mass.s == 0.0f ? 0.0f : 1.0f / mass.s;
@@ -1666,7 +1695,7 @@ __global__ __launch_bounds__(kJoin) void k_join(Rows a, JoinArgs g) {
       const float p = target_mass(q.t, a.c, e.z, mass.z) * inv;
       if (p == 0.0f) continue;
       if (e.id >= 0 && e.id < a.v) ce -= p * log_p(a, logit<T>(a, r, e.id), m, l);
-      h -= p * (kLn2 * log2f(p));
+      h -= p * log_share(p);
     }
     ce = fold64(ce, Add{});
     h = fold64(h, Add{});
@@ -1782,7 +1811,7 @@ __global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
       __syncthreads();
     }
     if constexpr (kTarget) {
-      Mass mass{neg_inf(), 0.0f};
+      Mass mass{no_mass(g.t), 0.0f};
       float bad = 0.0f;
       int* const tag = reinterpret_cast<int*>(dq);
       for (int j = l16; j < g.t.k; j += 16) {
@@ -1820,7 +1849,7 @@ __global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
         if constexpr (kOp != kDistillGrad) {
           if (q != 0.0f) {
             if (in) ce -= q * log_p(a, logit<T>(a, r, e.id), m, l);
-            h -= q * (kLn2 * log2f(q));
+            h -= q * log_share(q);
           }
         }
         if (kGrad && in && clash == 0.0f) dq[e.id] = -scale * q;
@@ -1887,11 +1916,17 @@ __global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
 
 // ---- launches (one unit a type) ----
 
+// Static LDS, bytes (rounded up).
+template <class T, int kC, int kOp>
+constexpr int kWaveLds = kOp == kLogprobsTop ? kWaveCandidates * 16
+                         : kOp == kLogprobs  ? 0
+                                             : 64 * kC * kPer<T> * 4;
+constexpr int kRowsLds = 8 * 1024;
+
 struct Launch {
   Rows a;
   Parts pt;
-  dim3 grid;
-  int waves;       // 0: k_tiny; 1 with `wave` chunks: k_wave
+  int waves;       // 0: k_tiny
   int wave;        // chunks a lane of k_wave (1, 2 or 4), 0: k_rows
   int chunks;      // a lane of k_rows
   unsigned lds;    // dynamic, bytes

@@ -28,7 +28,6 @@ struct Plan {
   int wave;   // chunks a lane of k_wave, 0: k_rows
   int chunks;  // a lane of k_rows
   Parts pt;
-  dim3 grid;
 };
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -44,26 +43,14 @@ Parts split(int32_t v, int64_t parts) {
   return p;
 }
 
-// A workgroup goes over several rows (loading the next one early) once the
-// card is full: `resident` waves a compute unit, the rounds evened out.
-dim3 row_grid(int64_t n, const Plan& p, int resident) {
-  const int64_t most = std::max<int64_t>(1, int64_t{kCus} * std::max(1, resident / p.waves) / p.pt.parts);
-  const int64_t rounds = up(n, most);
-  return dim3(static_cast<unsigned>(up(n, rounds)), static_cast<unsigned>(p.pt.parts));
-}
-
 // Rows of at most four chunks a lane: 16 lanes or a wave each.
 bool short_rows(const Rows& a, int size, Plan* p) {
   const int64_t bytes = int64_t{a.v} * size;
   if (bytes > kWaveFew && a.v > kTinyMax) return false;
   p->pt = Parts{1, a.v};
-  if (a.v <= kTinyMax) {
-    p->grid = dim3(static_cast<unsigned>(std::min<int64_t>(up(a.n, kTinyRows), kCus * 8)));
-    return true;
-  }
+  if (a.v <= kTinyMax) return true;
   p->waves = 1;
   p->wave = bytes <= kKib ? 1 : bytes <= 2 * kKib ? 2 : 4;
-  p->grid = row_grid(a.n, *p, 24);
   return true;
 }
 
@@ -90,7 +77,6 @@ Plan sums_plan(const Rows& a, int size) {
     parts = std::max(parts, std::min(up(2 * kCus, a.n), bytes / (16 * kKib)));
   p.pt = split(a.v, std::min<int64_t>(parts, kMaxSplit));
   fit(a, int64_t{p.pt.part} * size, a.n * p.pt.parts < 4 * kCus, &p);
-  p.grid = row_grid(a.n, p, p.chunks == kChunks ? 16 : p.chunks == kMidChunks ? 20 : 28);
   return p;
 }
 
@@ -101,14 +87,13 @@ Plan grad_plan(const Rows& a, int size) {
   const int64_t bytes = int64_t{a.v} * size;
   p.pt = split(a.v, up(bytes, 64 * kKib));
   fit(a, int64_t{p.pt.part} * size, a.n * p.pt.parts < 4 * kCus, &p);
-  p.grid = row_grid(a.n, p, 16);
   return p;
 }
 
 int type_size(int dtype) { return dtype == OS_AZ_F32 ? 4 : 2; }
 
 Launch launch(const Rows& a, const Plan& p, void* stream) {
-  return Launch{a, p.pt, p.grid, p.waves, p.wave, p.chunks, 0, static_cast<hipStream_t>(stream)};
+  return Launch{a, p.pt, p.waves, p.wave, p.chunks, 0, static_cast<hipStream_t>(stream)};
 }
 
 // Each part's sums and top keys, and the rows' stats where a caller wants none.
@@ -240,7 +225,6 @@ int os_az_logprobs_async(const os_az_rows* rows, const void* actions, int32_t wi
       Launch c = launch(a, p, hip_stream);
       k.rows(c, top > 0 ? kLogprobsTop : kLogprobs, g);
       if (need == 0) return;
-      c.grid = dim3(static_cast<unsigned>(a.n));
       k.join(c, false, JoinArgs{g, DistillArgs{}, p.pt.parts});
     });
   });
@@ -306,7 +290,6 @@ int os_az_distill_async(const os_az_rows* rows, const os_az_target* target, cons
       // (the gradient's launch reads the row's sums: left behind the parts')
       if (!stats) g.stats = reinterpret_cast<float*>(lp.sums + a.n * p.pt.parts);
       k.rows(c, kLogprobs, lp);
-      c.grid = dim3(static_cast<unsigned>(a.n));
       k.join(c, true, JoinArgs{lp, g, p.pt.parts});
       if (!grad) return;
       const Plan q = grad_plan(a, size);

@@ -2,34 +2,67 @@
 #ifndef OS_POLICY_LAUNCH_H_
 #define OS_POLICY_LAUNCH_H_
 
+#include <algorithm>
+
 #include "os_policy.h"
 
 namespace osp {
 
+constexpr int kCus = 256;
+
+// Waves of a kernel that fit a SIMD by its registers (512 a lane, in eights).
+template <auto kKernel>
+int waves_per_simd() {
+  static const int n = [] {
+    hipFuncAttributes f;
+    if (hipFuncGetAttributes(&f, reinterpret_cast<const void*>(kKernel)) != hipSuccess) return 4;
+    return std::max(1, std::min(8, 512 / std::max(8, (f.numRegs + 7) / 8 * 8)));
+  }();
+  return n;
+}
+
+// A workgroup goes over several rows (loading the next one early) once the
+// card is full: as many as are resident, the rounds evened out.
+inline dim3 row_grid(const Launch& c, int per_simd, int lds) {
+  int blocks = std::max(1, 4 * per_simd / c.waves);
+  if (lds > 0) blocks = std::max(1, std::min(blocks, 160 * 1024 / lds));
+  const int64_t most = std::max<int64_t>(1, int64_t{kCus} * blocks / c.pt.parts);
+  const int64_t rounds = (c.a.n + most - 1) / most;
+  return dim3(static_cast<unsigned>((c.a.n + rounds - 1) / rounds), static_cast<unsigned>(c.pt.parts));
+}
+
 template <class T, int kOp, class G>
 void launch_rows(const Launch& c, const G& g) {
   if (c.waves == 0) {
-    hipLaunchKernelGGL((k_tiny<T, kOp>), c.grid, dim3(kTinyBlock), 0, c.stream, c.a, g);
+    const int64_t blocks = std::min<int64_t>((c.a.n + kTinyRows - 1) / kTinyRows, kCus * 8);
+    hipLaunchKernelGGL((k_tiny<T, kOp>), dim3(static_cast<unsigned>(blocks)), dim3(kTinyBlock), 0,
+                       c.stream, c.a, g);
     return;
   }
   if (c.wave != 0) {
-    const auto go = [&](auto mask) {
+    const auto go = [&](auto mask, auto chunks) {
       constexpr bool kMask = decltype(mask)::value;
-      if (c.wave == 1)
-        hipLaunchKernelGGL((k_wave<T, kMask, 1, kOp>), c.grid, dim3(64), 0, c.stream, c.a, g);
-      else if (c.wave == 2)
-        hipLaunchKernelGGL((k_wave<T, kMask, 2, kOp>), c.grid, dim3(64), 0, c.stream, c.a, g);
-      else
-        hipLaunchKernelGGL((k_wave<T, kMask, 4, kOp>), c.grid, dim3(64), 0, c.stream, c.a, g);
+      constexpr int kC = decltype(chunks)::value;
+      constexpr auto kernel = &k_wave<T, kMask, kC, kOp>;
+      hipLaunchKernelGGL(kernel, row_grid(c, waves_per_simd<kernel>(), kWaveLds<T, kC, kOp>),
+                         dim3(64), 0, c.stream, c.a, g);
     };
-    if (c.a.legal != nullptr) go(std::true_type{});
-    else go(std::false_type{});
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    constexpr std::integral_constant<int, 4> four;
+    const auto by_chunks = [&](auto mask) {
+      if (c.wave == one) go(mask, one);
+      else if (c.wave == two) go(mask, two);
+      else go(mask, four);
+    };
+    if (c.a.legal != nullptr) by_chunks(std::true_type{});
+    else by_chunks(std::false_type{});
     return;
   }
-  const dim3 block(64 * c.waves);
   const auto go = [&](auto mask, auto chunks) {
-    hipLaunchKernelGGL((k_rows<T, decltype(mask)::value, decltype(chunks)::value, kOp>), c.grid,
-                       block, c.lds, c.stream, c.a, c.pt, g);
+    constexpr auto kernel = &k_rows<T, decltype(mask)::value, decltype(chunks)::value, kOp>;
+    hipLaunchKernelGGL(kernel, row_grid(c, waves_per_simd<kernel>(), static_cast<int>(c.lds) + kRowsLds),
+                       dim3(64 * c.waves), c.lds, c.stream, c.a, c.pt, g);
   };
   constexpr std::integral_constant<int, kFewChunks> few;
   constexpr std::integral_constant<int, kMidChunks> mid;
@@ -61,8 +94,9 @@ void Kernels<T>::rows(const Launch& c, int op, const DistillArgs& g) {
 }
 template <class T>
 void Kernels<T>::join(const Launch& c, bool loss, const JoinArgs& g) {
-  if (loss) hipLaunchKernelGGL((k_join<T, true>), c.grid, dim3(kJoin), 0, c.stream, c.a, g);
-  else hipLaunchKernelGGL((k_join<T, false>), c.grid, dim3(kJoin), 0, c.stream, c.a, g);
+  const dim3 grid(static_cast<unsigned>(c.a.n));
+  if (loss) hipLaunchKernelGGL((k_join<T, true>), grid, dim3(kJoin), 0, c.stream, c.a, g);
+  else hipLaunchKernelGGL((k_join<T, false>), grid, dim3(kJoin), 0, c.stream, c.a, g);
 }
 
 }  // namespace osp
