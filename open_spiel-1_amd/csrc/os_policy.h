@@ -379,7 +379,7 @@ __device__ __forceinline__ Entry target_entry(const Target& t, int64_t r, int j)
   return e;
 }
 // Entries first, first + step, .. of a row (those below k; the others none):
-// every load is issued before one is waited for.  id -1: none or past the
+// every load is issued before one is waited for, and all are waited for here.  id -1: none or past the
 // actions (then bad); z: the value, -inf where there is no mass.
 template <int kCount>
 __device__ __forceinline__ void target_entries(const Target& t, int64_t r, int first, int step,
@@ -434,6 +434,71 @@ __device__ __forceinline__ void target_entries(const Target& t, int64_t r, int f
     z[i] = none ? no_mass(t) : z[i];
   });
 }
+// The same in two halves, as they lie in memory in between: nothing waits before
+// finish().
+template <int kCount>
+struct RawEntries {
+  int64_t id[kCount];
+  uint32_t z[kCount];
+
+  // (uniform: how many of the batches hold any entry)
+  __device__ __forceinline__ static int rounds(const Target& t, int step) {
+    return min(kCount, (t.k + step - 1) / step);
+  }
+  __device__ __forceinline__ void load(const Target& t, int64_t r, int first, int step) {
+    if (t.k == 0) return;
+    const int n = rounds(t, step);
+    const auto all = [&](auto f) {
+#pragma unroll
+      for (int i = 0; i < kCount; ++i)
+        if (i < n) f(i, min(first + i * step, t.k - 1));
+    };
+    if (t.ids == nullptr) {
+      all([&](int i, int j) { id[i] = j; });
+    } else if (t.wide) {
+      const int64_t* const p = static_cast<const int64_t*>(t.ids) + r * t.ids_ld;
+      all([&](int i, int j) { id[i] = p[j]; });
+    } else {
+      const int32_t* const p = static_cast<const int32_t*>(t.ids) + r * t.ids_ld;
+      all([&](int i, int j) { id[i] = static_cast<uint32_t>(p[j]); });
+    }
+    if (t.type == OS_AZ_LOGITS_BF16 || t.type == OS_AZ_LOGITS_F16) {
+      const uint16_t* const p = static_cast<const uint16_t*>(t.val) + r * t.val_ld;
+      all([&](int i, int j) { z[i] = p[j]; });
+    } else {
+      const uint32_t* const p = static_cast<const uint32_t*>(t.val) + r * t.val_ld;
+      all([&](int i, int j) { z[i] = p[j]; });
+    }
+  }
+  // id -1: none or past the v actions (then bad); z: the value, no_mass() where
+  // there is none.
+  __device__ __forceinline__ void finish(const Target& t, int first, int step, int v,
+                                         int (&out)[kCount], float (&value)[kCount],
+                                         float& bad) const {
+    const int n = rounds(t, step);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      out[i] = -1;
+      value[i] = no_mass(t);
+      if (i < n) {
+        float f = __uint_as_float(z[i]);
+        if (t.type == OS_AZ_LOGITS_BF16) f = __uint_as_float(z[i] << 16);
+        else if (t.type == OS_AZ_LOGITS_F16)
+          f = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(z[i])));
+        else if (t.type == OS_AZ_WEIGHTS_I32) f = static_cast<float>(static_cast<int32_t>(z[i]));
+        // (a 32-bit action's sign is found here, not before its load is waited for)
+        const int64_t a = t.ids != nullptr && !t.wide ? static_cast<int32_t>(id[i]) : id[i];
+        // (selects only: written with && and an if, the compiler of ROCm 7.2
+        // lost the weights' f <= 0 case)
+        const bool in = (first + i * step < t.k) & (a >= 0), past = a >= v;
+        const bool none = !in | (is_weights(t) & (f <= 0.0f));
+        bad = in & past ? 1.0f : bad;
+        out[i] = in & !past ? static_cast<int>(a) : -1;
+        value[i] = none ? no_mass(t) : f;
+      }
+    }
+  }
+};
 // Running (maximum, mass relative to it) of target entries.
 struct Mass {
   float z, s;
@@ -613,11 +678,42 @@ struct Dense {
   }
 };
 
-// ---- long rows ----
+// ---- a row's single values ----
 
 template <int kOp>
 using ArgsOf = std::conditional_t<kOp == kLogprobs || kOp == kLogprobsTop, LogprobArgs,
                                   std::conditional_t<kOp == kLogprobsGrad, LogprobGradArgs, DistillArgs>>;
+
+// Fetched a row ahead: a scalar load waited for where it is used would cost its
+// whole latency at the start of every row.
+template <int kOp>
+struct RowValues {
+  int64_t given;  // kLogprobs*: the given action, -1: none
+  float m, l;     // kLogprobsGrad, kDistillGrad: the stats
+  float gl, gh, entropy, weight;
+
+  __device__ __forceinline__ static RowValues at(const ArgsOf<kOp>& g, int64_t r) {
+    RowValues v{-1, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 1.0f};
+    if constexpr (kOp == kLogprobs || kOp == kLogprobsTop || kOp == kLogprobsGrad)
+      if (g.actions != nullptr) v.given = uniform_id(g.actions, g.wide, r);
+    if constexpr (kOp == kLogprobsGrad || kOp == kDistillGrad) {
+      v.m = uniform(g.stats, 2 * r);
+      v.l = uniform(g.stats, 2 * r + 1);
+    }
+    if constexpr (kOp == kLogprobsGrad) {
+      if (g.gl != nullptr) v.gl = uniform(g.gl, r * g.gls);
+      if (g.gh != nullptr) {
+        v.gh = uniform(g.gh, r * g.ghs);
+        v.entropy = uniform(g.entropy, r);
+      }
+    }
+    if constexpr (kOp == kDistillFused || kOp == kDistillGrad)
+      if (g.weight != nullptr) v.weight = uniform(g.weight, r * g.weight_stride);
+    return v;
+  }
+};
+
+// ---- long rows ----
 
 // One workgroup of `nw` waves a row (or a part of one), kN chunks of 16 bytes a
 // lane.  kN = kFewChunks serves short rows, and few rows with more waves each;
@@ -696,6 +792,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     __syncthreads();
   }
 
+  RowValues<kOp> next = RowValues<kOp>::at(g, r);
+  RawEntries<kTarget ? kHeld : 1> next_entries;
+  if constexpr (kTarget) next_entries.load(g.t, r, tid, bd);
+
   for (int par = 0; r < a.n; r += gridDim.x, par ^= 1) {
     // The next row, loaded as this one's registers come free (after the last
     // row: one chunk, again and again).
@@ -705,7 +805,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     const uint8_t* const nl = kMask ? lb + rn * a.lld : nullptr;
     const int nlast = more ? len - kE : 0;
 
-    // -- listed entries: load, and their mass --
+    const RowValues<kOp> val = next;
+    next = RowValues<kOp>::at(g, rn);
+
+    // -- listed entries, and their mass --
     int eid[kTarget ? kHeld : 1];
     float ez[kTarget ? kHeld : 1], ex[kTarget ? kHeld : 1];
     Mass mass{neg_inf(), 0.0f};
@@ -713,7 +816,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     Table tab{};
     if constexpr (kTarget) {
       const int k = g.t.k;
-      target_entries<kHeld>(g.t, r, tid, bd, a.v, eid, ez, bad);
+      next_entries.finish(g.t, tid, bd, a.v, eid, ez, bad);
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) ex[i] = neg_inf();
       mass = mass_of(g.t, a.c, ez);
@@ -725,6 +828,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
 #pragma unroll
       for (int i = 0; i < kHeld; ++i)
         if (i * bd < k && eid[i] >= 0) ex[i] = logit<T>(a, r, eid[i]);
+      // (ahead of the next row's chunks: loads come back in order)
+      next_entries.load(g.t, rn, tid, bd);
       if constexpr (kGrad) {
         unsigned char* const base = dyn + static_cast<size_t>(par) * g.hash * 12;
         tab.key = reinterpret_cast<int32_t*>(base);
@@ -737,10 +842,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     }
 
     // -- the given action's logit --
-    int64_t given = -1;
+    const int64_t given = val.given;
     float given_x = neg_inf();
     if constexpr (kEnt || kOp == kLogprobsGrad) {
-      if (g.actions != nullptr) given = uniform_id(g.actions, g.wide, r);
       if (given >= 0 && given < a.v) given_x = logit<T>(a, r, given);
     }
 
@@ -877,8 +981,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
       m = u.m == neg_inf() ? 0.0f : u.m;
       l = u.s == 0.0f ? 0.0f : log2f(u.s);
     } else {
-      m = uniform(g.stats, 2 * r);
-      l = uniform(g.stats, 2 * r + 1);
+      m = val.m;
+      l = val.l;
     }
 
     // -- log probabilities --
@@ -1010,7 +1114,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     if constexpr (kTarget) {
       inv = mass.s == 0.0f ? 0.0f : 1.0f / mass.s;
       if constexpr (kGrad) {
-        scale = (g.weight != nullptr ? uniform(g.weight, r * g.weight_stride) : 1.0f) * a.inv_t;
+        scale = val.weight * a.inv_t;
         f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
       }
       float ce = 0.0f, h = 0.0f;
@@ -1071,7 +1175,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     if constexpr (kOp == kLogprobsGrad) {
       float sum = 0.0f;
       if (g.gl != nullptr && given >= 0) {
-        sum = given >= a.v ? __builtin_nanf("") : uniform(g.gl, r * g.gls);
+        sum = given >= a.v ? __builtin_nanf("") : val.gl;
         if (given < a.v) {
           act = static_cast<int>(given);
           act_w = sum * a.inv_t;
@@ -1099,9 +1203,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
           if (x > neg_inf() && !table_put(tab, static_cast<int>(ti), gt * a.inv_t, x)) twice[par] = 1;
         }
       }
-      const float gh = g.gh != nullptr ? uniform(g.gh, r * g.ghs) : 0.0f;
-      f0 = -(sum + (gh != 0.0f ? gh * uniform(g.entropy, r) : 0.0f)) * a.inv_t;
-      f1 = -gh * kLn2 * a.inv_t;
+      f0 = -(sum + (val.gh != 0.0f ? val.gh * val.entropy : 0.0f)) * a.inv_t;
+      f1 = -val.gh * kLn2 * a.inv_t;
     }
 
     // -- the gradient --
@@ -1202,14 +1305,22 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
 // are under way while a row is worked on.  No barrier is needed: what goes
 // through LDS stays within the wave, whose accesses are in order (fence() keeps
 // the compiler to it).
+// Waves a SIMD that the registers must leave room for (left alone, the compiler
+// keeps every address it could compute again): latency is hidden by waves here.
+template <bool kMask, int kX, int kOp>
+constexpr int kWaveRoom = kOp == kLogprobs || kOp == kLogprobsTop ? (kX <= 16 ? 6 : 4)
+                          : kOp == kDistill                       ? (kX <= 8 ? 6 : kX == 16 ? 5 : 4)
+                          : kX <= 8                               ? (kMask ? 4 : 5)
+                          : kX == 16                              ? 4
+                                                                  : 2;
 template <class T, bool kMask, int kC, int kOp>
-__global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
+__global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_wave(Rows a, ArgsOf<kOp> g) {
   constexpr int kE = kPer<T>, kX = kC * kE;
   constexpr bool kSums = kOp != kLogprobsGrad && kOp != kDistillGrad;
   constexpr bool kGrad = kOp == kLogprobsGrad || kOp == kDistillGrad || kOp == kDistillFused;
   constexpr bool kLp = kOp == kLogprobs || kOp == kLogprobsTop;
   constexpr bool kTarget = kOp == kDistill || kOp == kDistillFused || kOp == kDistillGrad;
-  constexpr int kHeld = 8;  // target entries a lane keeps in registers
+  constexpr int kHeld = 6;  // target entries a lane keeps in registers
   using Word = MaskWord<kE>;
   // The row's values, then its listed weights: chunk (t, lane) at
   // (t * 64 + lane) * kE, the row's last actions where their chunk has them.
@@ -1242,6 +1353,7 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
 #pragma unroll
   for (int t = kC / 2; t < kC; ++t) drop[t - kC / 2] = (t * 64 + lane) * kE - min((t * 64 + lane) * kE, last);
 
+  RowValues<kOp> next = RowValues<kOp>::at(g, blockIdx.x);
   load(blockIdx.x);
   for (int64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
     // -- the row's values --
@@ -1266,10 +1378,10 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       }
     }
     // -- what else the row needs from memory, ahead of the next row's loads --
-    int64_t given = -1;
+    const RowValues<kOp> val = next;
+    const int64_t given = val.given;
     float given_x = neg_inf();
     if constexpr (kLp || kOp == kLogprobsGrad) {
-      if (g.actions != nullptr) given = uniform_id(g.actions, g.wide, r);
       if (given >= 0 && given < a.v) given_x = logit<T>(a, r, given);
     }
     int eid[kTarget ? kHeld : 1];
@@ -1282,7 +1394,10 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
     if constexpr (kTarget) {
       target_entries<kHeld>(g.t, r, lane, 64, a.v, eid, ez, bad);
     }
-    if (r + gridDim.x < a.n) load(r + gridDim.x);
+    if (r + gridDim.x < a.n) {
+      next = RowValues<kOp>::at(g, r + gridDim.x);
+      load(r + gridDim.x);
+    }
 
     // -- the sums --
     float m, l, mean = 0.0f, lane_max = neg_inf();
@@ -1315,8 +1430,8 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       l = s == 0.0f ? 0.0f : log2f(s) - off;
       if constexpr (kLp) mean = s == 0.0f ? 0.0f : fold64(u, Add{}) / s - off;
     } else {
-      m = uniform(g.stats, 2 * r);
-      l = uniform(g.stats, 2 * r + 1);
+      m = val.m;
+      l = val.l;
     }
 
     if constexpr (kLp) {
@@ -1453,7 +1568,7 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       const float inv = mass.s == 0.0f ? 0.0f : 1.0f / mass.s;
       float scale = 0.0f, ce = 0.0f, h = 0.0f;
       if constexpr (kGrad) {
-        scale = (g.weight != nullptr ? uniform(g.weight, r * g.weight_stride) : 1.0f) * a.inv_t;
+        scale = val.weight * a.inv_t;
         f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
       }
       float ew[kGrad ? kHeld : 1];  // the weights, until the values are read
@@ -1532,7 +1647,7 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
     }
     if constexpr (kOp == kLogprobsGrad) {
       const bool in = g.gl != nullptr && given >= 0 && given < a.v;
-      const float gl = in ? uniform(g.gl, r * g.gls) : 0.0f;
+      const float gl = in ? val.gl : 0.0f;
       float sum = g.gl != nullptr && given >= a.v ? __builtin_nanf("") : gl;
       clear();
       fence();
@@ -1562,9 +1677,8 @@ __global__ __launch_bounds__(64) void k_wave(Rows a, ArgsOf<kOp> g) {
       }
       if (lane == 0 && in && given_x > neg_inf()) row[slot(static_cast<int>(given))] += gl * a.inv_t;
       fence();
-      const float gh = g.gh != nullptr ? uniform(g.gh, r * g.ghs) : 0.0f;
-      f0 = -(sum + (gh != 0.0f ? gh * uniform(g.entropy, r) : 0.0f)) * a.inv_t;
-      f1 = -gh * kLn2 * a.inv_t;
+      f0 = -(sum + (val.gh != 0.0f ? val.gh * val.entropy : 0.0f)) * a.inv_t;
+      f1 = -val.gh * kLn2 * a.inv_t;
     }
 
     // -- the gradient --
