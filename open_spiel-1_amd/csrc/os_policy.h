@@ -156,15 +156,18 @@ __device__ __forceinline__ float get(const _Float16* p, int64_t i) { return stat
 
 // Rows start anywhere their type may (an odd row stride, a view's column
 // offset): wide accesses are declared with the element's alignment only.
-template <class T, class W>
+// kStream: read or written once (a hint to the caches).
+template <bool kStream, class T, class W>
 __device__ __forceinline__ W load_at(const T* p) {
-  struct __attribute__((packed, aligned(sizeof(T)))) P { W w; };
-  return reinterpret_cast<const P*>(p)->w;
+  typedef W Any __attribute__((aligned(sizeof(T))));
+  if constexpr (kStream) return __builtin_nontemporal_load(reinterpret_cast<const Any*>(p));
+  else return *reinterpret_cast<const Any*>(p);
 }
-template <class T, class W>
+template <bool kStream, class T, class W>
 __device__ __forceinline__ void store_at(T* p, W w) {
-  struct __attribute__((packed, aligned(sizeof(T)))) P { W w; };
-  reinterpret_cast<P*>(p)->w = w;
+  typedef W Any __attribute__((aligned(sizeof(T))));
+  if constexpr (kStream) __builtin_nontemporal_store(w, reinterpret_cast<Any*>(p));
+  else *reinterpret_cast<Any*>(p) = w;
 }
 
 // A chunk's mask bytes.
@@ -551,12 +554,15 @@ __device__ __forceinline__ uint64_t fold64_max(uint64_t v) {
 // element from below.  Bisection between the least and the largest, counting
 // with ballots on the scalar unit: six steps or so, where ranking every lane
 // against every other takes 192 vector operations.
-__device__ __forceinline__ float kth_bound(float v, int k) {
+// `most` is the lanes' largest; kExact: the bound is a lane's value.
+template <bool kExact>
+__device__ __forceinline__ float kth_bound(float v, float most, int k) {
+  if (k == 1) return most;
   const float inf = __builtin_huge_valf();
   const bool any = v > neg_inf();
   if (__builtin_popcountll(__ballot(any)) < k) return neg_inf();
   float lo = -fold64(any ? -v : -inf, Max{});
-  float hi = fold64(v, Max{});
+  float hi = most;
   const int enough = k + (k >> 2) + 3;
   for (int step = 0; step < 24; ++step) {
     const float mid = fmaf(lo, 0.5f, hi * 0.5f);
@@ -566,7 +572,7 @@ __device__ __forceinline__ float kth_bound(float v, int k) {
     else hi = mid;
     if (n >= k && n <= enough) break;
   }
-  return -fold64(v >= lo ? -v : -inf, Max{});
+  return kExact ? -fold64(v >= lo ? -v : -inf, Max{}) : lo;
 }
 
 // The k-th largest (k >= 1) of one key a lane.
@@ -718,7 +724,9 @@ struct RowValues {
 // One workgroup of `nw` waves a row (or a part of one), kN chunks of 16 bytes a
 // lane.  kN = kFewChunks serves short rows, and few rows with more waves each;
 // the longest rows take 16 (8 with a mask, whose bytes want registers too).
-template <class T, bool kMask, int kN, int kOp>
+// kStream: the logits exceed the last-level cache, so nothing of them is worth
+// keeping there (131072 bf16 actions x 2048 rows, 64 targets: 268 -> 253 us).
+template <class T, bool kMask, int kN, int kOp, bool kStream>
 __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsOf<kOp> g) {
   constexpr int kE = kPer<T>;
   constexpr bool kSums = kOp != kLogprobsGrad && kOp != kDistillGrad;
@@ -752,9 +760,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     // (an unsigned byte offset to a uniform base: no 64-bit address arithmetic)
     const uint32_t oc = min((t * bd + me) * kE, last);
     const uint32_t bytes = oc * static_cast<uint32_t>(sizeof(T));
-    raw[t] = load_at<T, u32x4>(
+    raw[t] = load_at<kStream, T, u32x4>(
         reinterpret_cast<const T*>(reinterpret_cast<const char*>(x) + bytes));
-    if constexpr (kMask) mk[t] = load_at<uint8_t, Word>(legal + oc);
+    if constexpr (kMask) mk[t] = *reinterpret_cast<const Word*>(legal + oc);
   };
   // The chunk's values, excluded ones -inf; true where it holds any.
   auto values = [&](int t, float (&x)[kE], int ln) {
@@ -1015,7 +1023,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
           const uint64_t key = nw == 1 ? lane_key : top_lds.group[lane];
           const float v = key == 0 ? neg_inf() : key_value(key);
           const int at = key == 0 ? 0x7FFFFFFF : static_cast<int>(key_index(key));
-          const float tv = kth_bound(v, g.top);
+          const float tv = kth_bound<true>(v, m, g.top);
           // of those at the bound, as many as `top` still needs, the first
           const uint64_t tied = __ballot(v == tv && key != 0);
           const int need = g.top - __builtin_popcountll(__ballot(v > tv));
@@ -1117,6 +1125,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
         scale = val.weight * a.inv_t;
         f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
       }
+    }
+    // The entries' part in the loss, and their weights into the table (before the
+    // gradient's pass, whose loads for the next row the logits' would wait for).
+    [[maybe_unused]] const auto use_targets = [&](const auto& g) {
       float ce = 0.0f, h = 0.0f;
       const auto use = [&](int id, float z, float x) {
         const float q = target_mass(g.t, a.c, z, mass.z) * inv;
@@ -1142,31 +1154,30 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
       if constexpr (kOp != kDistillGrad) {
         ce = fold64(ce, Add{});
         h = fold64(h, Add{});
-        const auto out = [&] {
-          g.loss[r] = bad != 0.0f ? __builtin_nanf("") : ce;
-          if (g.tent != nullptr) g.tent[r] = h;
-          if (g.stats != nullptr) {
-            g.stats[2 * r] = m;
-            g.stats[2 * r + 1] = l;
-          }
-        };
-        if (nw == 1) {
-          if (tid == 0) out();
-        } else {
-          if (lane == 0) {
-            red2[par][wave][0] = ce;
-            red2[par][wave][1] = h;
-          }
-          __syncthreads();
-          if (tid == 0) {
-            for (int w = 1; w < nw; ++w) {
-              ce += red2[par][w][0];
-              h += red2[par][w][1];
-            }
-            out();
-          }
+        if (lane == 0) {
+          red2[par][wave][0] = ce;
+          red2[par][wave][1] = h;
         }
       }
+    };
+    [[maybe_unused]] const auto write_loss = [&](const auto& g) {  // after the barrier
+      if (tid != 0) return;
+      float ce = 0.0f, h = 0.0f;
+      for (int w = 0; w < nw; ++w) {
+        ce += red2[par][w][0];
+        h += red2[par][w][1];
+      }
+      g.loss[r] = bad != 0.0f ? __builtin_nanf("") : ce;
+      if (g.tent != nullptr) g.tent[r] = h;
+      if (g.stats != nullptr) {
+        g.stats[2 * r] = m;
+        g.stats[2 * r + 1] = l;
+      }
+    };
+    if constexpr (kTarget) use_targets(g);
+    if constexpr (kOp == kDistill) {
+      __syncthreads();
+      write_loss(g);
     }
 
     // -- gradient of the log probabilities: factors and listed weights --
@@ -1229,7 +1240,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
           }
           if (o + kE <= ln) {
             const uint32_t bytes = static_cast<uint32_t>(o) * static_cast<uint32_t>(sizeof(T));
-            store_at<T>(reinterpret_cast<T*>(reinterpret_cast<char*>(gb) + bytes), pack<T>(y));
+            store_at<kStream>(reinterpret_cast<T*>(reinterpret_cast<char*>(gb) + bytes), pack<T>(y));
           } else if (o < ln) {
 #pragma unroll
             for (int j = 0; j < kE; ++j)
@@ -1245,6 +1256,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
       };
       if constexpr (kTarget) {
         __syncthreads();
+        if constexpr (kOp == kDistillFused) write_loss(g);
         if (twice[par] != 0) {
           // the entries in order, through the other row's table (at rest)
           unsigned char* const base = dyn + static_cast<size_t>(par ^ 1) * g.hash * 12;
@@ -1339,8 +1351,8 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_w
 #pragma unroll
     for (int t = 0; t < kC; ++t) {
       const int oc = min((t * 64 + lane) * kE, last);
-      raw[t] = load_at<T, u32x4>(x + oc);
-      if constexpr (kMask) mk[t] = load_at<uint8_t, Word>(legal + oc);
+      raw[t] = load_at<false, T, u32x4>(x + oc);
+      if constexpr (kMask) mk[t] = *reinterpret_cast<const Word*>(legal + oc);
     }
   };
   // Where an action is in `row`: the last, shifted chunk holds those from
@@ -1456,7 +1468,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_w
         g.top_logprob[r * g.top + rank] =
             odd ? l : key == 0 ? neg_inf() : log_p(a, key_value(key), m, l);
       };
-      const float bound = fmaxf(kth_bound(lane_max, g.top), kLowest);
+      const float bound = fmaxf(kth_bound<false>(lane_max, m, g.top), kLowest);
       int found = 0;
       renew(me);
       if (!odd) {
@@ -1701,7 +1713,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_w
         }
         const int o = (t * 64 + me) * kE;
         if (t < kC / 2 || o + kE <= a.v) {
-          store_at<T>(gb + o, pack<T>(y));
+          store_at<false>(gb + o, pack<T>(y));
         } else if (o < a.v) {
 #pragma unroll
           for (int j = 0; j < kE; ++j)
@@ -2043,6 +2055,7 @@ struct Launch {
   int waves;       // 0: k_tiny
   int wave;        // chunks a lane of k_wave (1, 2 or 4), 0: k_rows
   int chunks;      // a lane of k_rows
+  bool streamed;   // k_rows: see kStream
   unsigned lds;    // dynamic, bytes
   hipStream_t stream;
 };

@@ -17,6 +17,7 @@ using namespace osp;
 
 constexpr int kCus = 256;
 constexpr int64_t kKib = 1024;
+constexpr int64_t kLastLevelCache = int64_t{256} << 20;
 constexpr int64_t kWaveFew = kFewChunks * kKib;  // bytes a wave holds: 64 lanes x 16 a chunk
 // (sums_plan leaves rows of up to four such waves whole)
 static_assert(OS_AZ_NO_WORKSPACE_ACTIONS * 4 <= 4 * kWaveFew);
@@ -27,6 +28,7 @@ struct Plan {
   int waves;  // 0: k_tiny
   int wave;   // chunks a lane of k_wave, 0: k_rows
   int chunks;  // a lane of k_rows
+  bool streamed;  // k_rows does not ask the caches to keep the logits
   Parts pt;
 };
 
@@ -59,12 +61,17 @@ int64_t wave_bytes(const Rows& a) { return (a.legal ? kMidChunks : kChunks) * kK
 // Chunks a lane and waves for `bytes` a workgroup: with `wide` as many waves
 // as four chunks each allow (few rows: each is over sooner), else as few as the
 // registers allow (more rows at once, fewer waves to join).
-void fit(const Rows& a, int64_t bytes, bool wide, Plan* p) {
+void fit(const Rows& a, int size, int64_t bytes, bool wide, Plan* p) {
   const int64_t most = wave_bytes(a);
   if (wide && bytes <= kMaxWaves * kWaveFew) p->chunks = kFewChunks;
-  else if (bytes <= kMidChunks * kKib || most == kMidChunks * kKib) p->chunks = kMidChunks;
+  else if (bytes <= kChunks * kKib || most == kMidChunks * kKib) p->chunks = kMidChunks;
   else p->chunks = kChunks;
   p->waves = static_cast<int>(up(bytes, p->chunks * kKib));
+  // (16-bit rows that start between dwords share their lines' ends with their
+  // neighbours: dropped early, those are read twice - 50021 bf16 actions x 2048
+  // rows, log probabilities: 42 us kept, 51 us dropped)
+  p->streamed = p->chunks == kChunks && a.n * a.v * size > kLastLevelCache &&
+              (size == 4 || ((reinterpret_cast<uintptr_t>(a.x) | (a.ld * size)) & 3) == 0);
 }
 
 // Kernels that need the row's sums.
@@ -76,7 +83,7 @@ Plan sums_plan(const Rows& a, int size) {
   if (a.n < 2 * kCus && bytes > 4 * kWaveFew)
     parts = std::max(parts, std::min(up(2 * kCus, a.n), bytes / (16 * kKib)));
   p.pt = split(a.v, std::min<int64_t>(parts, kMaxSplit));
-  fit(a, int64_t{p.pt.part} * size, a.n * p.pt.parts < 4 * kCus, &p);
+  fit(a, size, int64_t{p.pt.part} * size, a.n * p.pt.parts < 4 * kCus, &p);
   return p;
 }
 
@@ -86,14 +93,14 @@ Plan grad_plan(const Rows& a, int size) {
   if (short_rows(a, size, &p)) return p;
   const int64_t bytes = int64_t{a.v} * size;
   p.pt = split(a.v, up(bytes, 64 * kKib));
-  fit(a, int64_t{p.pt.part} * size, a.n * p.pt.parts < 4 * kCus, &p);
+  fit(a, size, int64_t{p.pt.part} * size, a.n * p.pt.parts < 4 * kCus, &p);
   return p;
 }
 
 int type_size(int dtype) { return dtype == OS_AZ_F32 ? 4 : 2; }
 
 Launch launch(const Rows& a, const Plan& p, void* stream) {
-  return Launch{a, p.pt, p.waves, p.wave, p.chunks, 0, static_cast<hipStream_t>(stream)};
+  return Launch{a, p.pt, p.waves, p.wave, p.chunks, p.streamed, 0, static_cast<hipStream_t>(stream)};
 }
 
 // Each part's sums and top keys, and the rows' stats where a caller wants none.

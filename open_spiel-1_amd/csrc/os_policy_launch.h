@@ -59,21 +59,25 @@ void launch_rows(const Launch& c, const G& g) {
     else by_chunks(std::false_type{});
     return;
   }
-  const auto go = [&](auto mask, auto chunks) {
-    constexpr auto kernel = &k_rows<T, decltype(mask)::value, decltype(chunks)::value, kOp>;
+  const auto go = [&](auto mask, auto chunks, auto stream) {
+    constexpr auto kernel =
+        &k_rows<T, decltype(mask)::value, decltype(chunks)::value, kOp, decltype(stream)::value>;
     hipLaunchKernelGGL(kernel, row_grid(c, waves_per_simd<kernel>(), static_cast<int>(c.lds) + kRowsLds),
                        dim3(64 * c.waves), c.lds, c.stream, c.a, c.pt, g);
   };
   constexpr std::integral_constant<int, kFewChunks> few;
   constexpr std::integral_constant<int, kMidChunks> mid;
   constexpr std::integral_constant<int, kChunks> many;
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
   if (c.a.legal != nullptr) {
-    if (c.chunks == few) go(std::true_type{}, few);
-    else go(std::true_type{}, mid);
+    if (c.chunks == few) go(yes, few, no);
+    else go(yes, mid, no);
   } else {
-    if (c.chunks == few) go(std::false_type{}, few);
-    else if (c.chunks == mid) go(std::false_type{}, mid);
-    else go(std::false_type{}, many);
+    if (c.chunks == few) go(no, few, no);
+    else if (c.chunks == mid) go(no, mid, no);
+    else if (c.streamed) go(no, many, yes);
+    else go(no, many, no);
   }
 }
 
