@@ -376,7 +376,7 @@ int os_az_mlp_heads_async(const float* obs, int64_t num_rows, int32_t obs_size,
 #define OS_AZ_BF16 1
 #define OS_AZ_F16 2
 #define OS_AZ_MAX_ACTIONS 2097152
-#define OS_AZ_NO_WORKSPACE_ACTIONS 4096 /* rows of up to this many need none */
+#define OS_AZ_NO_WORKSPACE_ACTIONS 32768 /* rows of up to this many need none */
 #define OS_AZ_MAX_TOP 64
 #define OS_AZ_MAX_TARGETS 1024
 typedef struct os_az_rows {

@@ -19,8 +19,9 @@ constexpr int kCus = 256;
 constexpr int64_t kKib = 1024;
 constexpr int64_t kLastLevelCache = int64_t{256} << 20;
 constexpr int64_t kWaveFew = kFewChunks * kKib;  // bytes a wave holds: 64 lanes x 16 a chunk
-// (sums_plan leaves rows of up to four such waves whole)
-static_assert(OS_AZ_NO_WORKSPACE_ACTIONS * 4 <= 4 * kWaveFew);
+// (sums_plan leaves rows that fit a workgroup whole, masked or not)
+constexpr int64_t kWholeRow = kMaxWaves * kMidChunks * kKib;
+static_assert(OS_AZ_NO_WORKSPACE_ACTIONS * 4 <= kWholeRow);
 
 // ---- how the workgroups share the rows ----
 
@@ -58,13 +59,15 @@ bool short_rows(const Rows& a, int size, Plan* p) {
 
 int64_t wave_bytes(const Rows& a) { return (a.legal ? kMidChunks : kChunks) * kKib; }
 
-// Chunks a lane and waves for `bytes` a workgroup: with `wide` as many waves
-// as four chunks each allow (few rows: each is over sooner), else as few as the
-// registers allow (more rows at once, fewer waves to join).
+// Chunks a lane and waves for `bytes` a workgroup: with `wide` as many waves as
+// a workgroup has (few rows: each is over sooner), else as few as the registers
+// allow (more rows at once, fewer waves to join; 8 chunks up to 16 KiB, where
+// listed actions are read again and 16 would crowd them out of the cache).
 void fit(const Rows& a, int size, int64_t bytes, bool wide, Plan* p) {
   const int64_t most = wave_bytes(a);
   if (wide && bytes <= kMaxWaves * kWaveFew) p->chunks = kFewChunks;
-  else if (bytes <= kChunks * kKib || most == kMidChunks * kKib) p->chunks = kMidChunks;
+  else if (bytes <= (wide ? kMaxWaves * kMidChunks : kChunks) * kKib || most == kMidChunks * kKib)
+    p->chunks = kMidChunks;
   else p->chunks = kChunks;
   p->waves = static_cast<int>(up(bytes, p->chunks * kKib));
   // (16-bit rows that start between dwords share their lines' ends with their
@@ -79,9 +82,12 @@ Plan sums_plan(const Rows& a, int size) {
   Plan p{};
   if (short_rows(a, size, &p)) return p;
   const int64_t bytes = int64_t{a.v} * size, most = kMaxWaves * wave_bytes(a);
+  // A row in one workgroup as long as it fits: joining parts costs a launch and
+  // the gradient a second read.  Only few rows near that limit are over sooner
+  // in parts (131072 bf16 actions, top 20: 1 row 13 us in parts, 17 whole; 128
+  // rows 22 and 19; 65536 actions: 1 row 12.5 and 12, 256 rows 22 and 14).
   int64_t parts = up(bytes, most);
-  if (a.n < 2 * kCus && bytes > 4 * kWaveFew)
-    parts = std::max(parts, std::min(up(2 * kCus, a.n), bytes / (16 * kKib)));
+  if (a.n <= 64 && bytes > kWholeRow) parts = std::max(parts, bytes / (16 * kKib));
   p.pt = split(a.v, std::min<int64_t>(parts, kMaxSplit));
   fit(a, size, int64_t{p.pt.part} * size, a.n * p.pt.parts < 4 * kCus, &p);
   return p;

@@ -215,7 +215,7 @@ _sig("os_az_distill_grad_async", ctypes.c_int,
 AZ_F32, AZ_BF16, AZ_F16 = 0, 1, 2
 AZ_LOGITS_F32, AZ_LOGITS_BF16, AZ_LOGITS_F16, AZ_WEIGHTS_F32, AZ_WEIGHTS_I32 = range(5)
 AZ_MAX_ACTIONS, AZ_MAX_TOP, AZ_MAX_TARGETS = 2097152, 64, 1024
-AZ_NO_WORKSPACE_ACTIONS = 4096
+AZ_NO_WORKSPACE_ACTIONS = 32768
 AZ_ROWS_BYTES, AZ_TARGET_BYTES = ctypes.sizeof(AzRows), ctypes.sizeof(AzTarget)
 _sig("os_az_fetch", ctypes.c_int, [_vp, _i32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P])
 _sig("os_engine_node_bytes", _i32, [_vp])
