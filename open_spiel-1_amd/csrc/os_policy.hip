@@ -86,7 +86,8 @@ Plan sums_plan(const Rows& a, int size) {
   // the gradient a second read.  Only few rows near that limit are over sooner
   // in parts (131072 bf16 actions, top 20: 1 row 13 us in parts, 17 whole; 128
   // rows 22 and 19; 65536 actions: 1 row 12.5 and 12, 256 rows 22 and 14).
-  int64_t parts = up(bytes, most);
+  // Rows that do not fit go in parts of 64 KiB, four workgroups a compute unit.
+  int64_t parts = bytes <= most ? 1 : up(bytes, 64 * kKib);
   if (a.n <= 64 && bytes > kWholeRow) parts = std::max(parts, bytes / (16 * kKib));
   p.pt = split(a.v, std::min<int64_t>(parts, kMaxSplit));
   fit(a, size, int64_t{p.pt.part} * size, a.n * p.pt.parts < 4 * kCus, &p);
