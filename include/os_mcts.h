@@ -367,8 +367,9 @@ int os_az_mlp_heads_async(const float* obs, int64_t num_rows, int32_t obs_size,
  * its action too.  With x = logit / temperature on the remaining actions,
  * p = softmax(x).  A row without any is empty: p = 0, gradient 0.  A NaN or
  * +inf logit on a legal action makes its row's results NaN and no other row's.
- * Logits f32, bf16 or f16 (dtype); arithmetic and results f32; gradients are
- * rounded once to the logits' type.  Buffers do not overlap.  Every call
+ * Logits f32, bf16 or f16 (dtype); arithmetic and results f32 (a probability
+ * below 2^-126 times the row's largest counts as 0); gradients are rounded once
+ * to the logits' type.  Buffers do not overlap.  Every call
  * launches on hip_stream, whose device must be current, allocates nothing and
  * may be captured; it reads no device data on the host, so what ids hold is
  * checked on the device, as said with each. */
@@ -387,7 +388,7 @@ typedef struct os_az_rows {
   int64_t legal_ld;     /* legal row stride, bytes */
   int32_t num_actions;  /* 1 .. OS_AZ_MAX_ACTIONS */
   int32_t dtype;        /* OS_AZ_F32 / _BF16 / _F16 */
-  float temperature;    /* > 0, finite */
+  float temperature;    /* 1e-30 .. 1e30 */
   int32_t reserved;     /* 0 */
 } os_az_rows;
 /* A target distribution on k listed actions of each row: entry j of row r is

@@ -35,8 +35,8 @@
 namespace osp {
 
 constexpr float kLn2 = 0.69314718055994530942f;
-// d below this is e = 0 in f32 (2^-149 is the least subnormal): keeps 0 * -inf
-// out of the sums.
+// 2^d is 0 here (the exponential keeps no subnormals: from -126 down): keeps
+// 0 * -inf out of the sums.
 constexpr float kFloor = -160.0f;
 // Rows whose maximum times c is further out than this ("wild") take the plain
 // form 2^((x - m) c): beyond it the rounding of m c alone would be over half a
@@ -48,9 +48,9 @@ constexpr int kMaxWaves = 16;
 constexpr int kMaxSplit = 64;      // parts of a row
 constexpr int kCandidates = 512;   // top actions: LDS list
 constexpr int kWaveCandidates = 256;  // of a wave alone (a multiple of 64)
-constexpr int kFewChunks = 4;      // chunks a lane in the kernels for short rows
-constexpr int kMidChunks = 8;      // for longer ones; the most with a mask
-constexpr int kChunks = 16;        // the most without
+constexpr int kFewChunks = 4;      // chunks a lane: the most of k_wave, the least of k_rows,
+constexpr int kMidChunks = 8;      // its most with a mask
+constexpr int kChunks = 16;        // and without
 
 struct Rows {
   const void* x;
@@ -382,8 +382,9 @@ __device__ __forceinline__ Entry target_entry(const Target& t, int64_t r, int j)
   return e;
 }
 // Entries first, first + step, .. of a row (those below k; the others none):
-// every load is issued before one is waited for, and all are waited for here.  id -1: none or past the
-// actions (then bad); z: the value, -inf where there is no mass.
+// every load is issued before one is waited for, and all are waited for here.
+// id -1: none or past the v actions (then bad); z: the value, no_mass() where
+// there is none.
 template <int kCount>
 __device__ __forceinline__ void target_entries(const Target& t, int64_t r, int first, int step,
                                                int v, int (&id)[kCount], float (&z)[kCount],
@@ -437,8 +438,9 @@ __device__ __forceinline__ void target_entries(const Target& t, int64_t r, int f
     z[i] = none ? no_mass(t) : z[i];
   });
 }
-// The same in two halves, as they lie in memory in between: nothing waits before
-// finish().
+// The same in two halves, as they lie in memory in between: load() issues every
+// load and finish() is the first to wait for one.  (Held across a row by k_rows;
+// k_wave's six entries a lane would spill as this form.)
 template <int kCount>
 struct RawEntries {
   int64_t id[kCount];
@@ -722,8 +724,9 @@ struct RowValues {
 // ---- long rows ----
 
 // One workgroup of `nw` waves a row (or a part of one), kN chunks of 16 bytes a
-// lane.  kN = kFewChunks serves short rows, and few rows with more waves each;
-// the longest rows take 16 (8 with a mask, whose bytes want registers too).
+// lane: kFewChunks where there are few rows (more waves each), kMidChunks or
+// kChunks where there are many; with a mask, whose bytes want registers too, at
+// most kMidChunks.
 // kStream: the logits exceed the last-level cache, so nothing of them is worth
 // keeping there (131072 bf16 actions x 2048 rows, 64 targets: 268 -> 253 us).
 template <class T, bool kMask, int kN, int kOp, bool kStream>
@@ -961,7 +964,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     }
     float m, l;
     if constexpr (kSums) {
-      if (u.m > neg_inf() && !(fabsf(u.m * a.c) <= kWild)) {
+      // (well within -kWild: a lane below it has summed against that, not
+      // against its own maximum, and must not count)
+      if (u.m > neg_inf() && !(fabsf(u.m * a.c) <= kWild - 256.0f)) {
         // a wild row: once more, from memory
         u.s = u.t = 0.0f;
         for (int i = tid; i < len; i += bd) {
@@ -1730,6 +1735,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_w
 // One workgroup of kJoin lanes a row: the parts' sums (a lane each), then their
 // top lists or the loss.
 constexpr int kJoin = 256;
+constexpr int kJoinGridX = 1 << 20;
 
 template <class T, bool kLoss>
 __global__ __launch_bounds__(kJoin) void k_join(Rows a, JoinArgs g) {
@@ -1737,7 +1743,9 @@ __global__ __launch_bounds__(kJoin) void k_join(Rows a, JoinArgs g) {
   __shared__ uint32_t count;
   __shared__ float red[kJoin / 64][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r = blockIdx.x;
+  // (a grid of more than 2^32 lanes along x is not launched)
+  const int64_t r = blockIdx.y * int64_t{kJoinGridX} + blockIdx.x;
+  if (r >= a.n) return;
   const PartSums* const ps = g.lp.sums + r * g.parts;
   Sums u{neg_inf(), 0.0f, 0.0f};
   if (lane < g.parts) u = Sums{ps[lane].m, ps[lane].s, ps[lane].t};

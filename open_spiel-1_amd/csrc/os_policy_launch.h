@@ -98,7 +98,8 @@ void Kernels<T>::rows(const Launch& c, int op, const DistillArgs& g) {
 }
 template <class T>
 void Kernels<T>::join(const Launch& c, bool loss, const JoinArgs& g) {
-  const dim3 grid(static_cast<unsigned>(c.a.n));
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(c.a.n, kJoinGridX)),
+                  static_cast<unsigned>((c.a.n + kJoinGridX - 1) / kJoinGridX));
   if (loss) hipLaunchKernelGGL((k_join<T, true>), grid, dim3(kJoin), 0, c.stream, c.a, g);
   else hipLaunchKernelGGL((k_join<T, false>), grid, dim3(kJoin), 0, c.stream, c.a, g);
 }

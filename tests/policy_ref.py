@@ -5,6 +5,10 @@ import math
 import torch
 
 U = 2.0 ** -24  # half a step of float32, relative
+# The gradients' p = e f is a float32 exponential e of (x - m) / T <= 0 times
+# f = 1 / sum e <= 1.  The exponential keeps no subnormal results: e < 2^-126 is
+# 0, so p is off by up to 2^-126 beside its relative error.
+LEAST = 2.0 ** -126
 
 
 def adds(v):
@@ -117,6 +121,8 @@ def logprobs_grad(logits, actions=None, legal=None, temperature=1.0, g_logprob=N
   k = 0 if not torch.is_tensor(ids) else ids.shape[1]
   bound = U * ((3 * adds(v) * (1 + math.log2(max(v, 2))) + 12 * span + k) * part
                + (k + 4) * amount)
+  # (p |log p| <= LEAST |log LEAST| < 104 LEAST where p <= LEAST)
+  bound = bound + LEAST * (size + gh.abs() * (104 + 1 + h[:, 0].abs()))[:, None]
   return grad / temperature, bound / temperature
 
 
@@ -180,7 +186,7 @@ def distill(logits, target, ids=None, legal=None, kind="weights", temperature=1.
   sp = torch.where(p > 0, (x - x.amax(1, keepdim=True)).abs(), torch.zeros_like(x))
   s = (w / temperature)[:, None]
   out["grad"] = grad * s
-  tol["grad"] = (p * U * (3 * adds(v) + 12 * sp + 16) + sq_err + 4 * U * sq) * s.abs()
+  tol["grad"] = (p * U * (3 * adds(v) + 12 * sp + 16) + sq_err + 4 * U * sq + LEAST) * s.abs()
   return out, tol
 
 

@@ -414,6 +414,151 @@ def test_gpu_many_rows(require_gpu, n, v):
   assert float((grad - want).abs().max()) < 3 * bound
 
 
+def held_there(got, want, tol, what):
+  """close() without leaving the GPU."""
+  want, tol, got = want.float().double(), tol.double(), got.detach().double()
+  ok = (got == want) | (torch.isnan(got) & torch.isnan(want)) | ((got - want).abs() <= tol)
+  if not bool(ok.all()):
+    i = tuple(int(k) for k in torch.nonzero(~ok)[0])
+    raise AssertionError("%s: %d of %d off, first at %s: %r, expected %r +- %r"
+                         % (what, int((~ok).sum()), ok.numel(), i, float(got[i]), float(want[i]),
+                            float(tol[i])))
+
+
+@gpu
+@pytest.mark.parametrize("n,v,k,dtype,masked", [
+    (1200, 2500, 1024, "f32", False), (1200, 2500, 600, "f32", True), (2600, 4099, 70, "f16", True),
+    (2600, 4099, 70, "bf16", False), (1100, 9001, 70, "f32", False), (1100, 9001, 300, "bf16", True),
+    (1030, 40000, 70, "bf16", False), (1030, 40001, 70, "f32", True), (1030, 70001, 9, "f32", False)])
+def test_gpu_many_long_rows(require_gpu, n, v, k, dtype, masked):
+  """Workgroups that go over several long rows, far ones, empty ones and ones
+  with actions listed twice among them (the 64-bit formulas on the GPU)."""
+  from os_amd import policy
+  g = torch.Generator(device="cuda").manual_seed(n + v + k)
+  f = dict(device="cuda", generator=g)
+  x = torch.randn(n, v, **f) * 2.5
+  x[7::97] += 30000.0
+  if dtype == "f32":
+    x[5::89] *= 2.0 ** 30
+  x = x.to(TYPES[dtype])
+  legal = None
+  if masked:
+    legal = (torch.rand(n, v, **f) < 0.6).to(torch.uint8)
+    legal[::71] = 0
+  actions = torch.randint(-1, v, (n,), **f)
+  ids = torch.randint(0, v, (n, k), **f)
+  ids[3::13, 1] = ids[3::13, 0]
+  ids[::3, k // 2] = -1
+  w = torch.rand(n, k, **f)
+  if masked:
+    w = w * legal.gather(1, ids.clamp(min=0))
+  weight = torch.randn(n, **f)
+  gl, gh, gt = torch.randn(n, **f), torch.randn(n, **f), torch.randn(n, 5, **f)
+  leaf = x.clone().requires_grad_()
+  r = policy.logprobs(leaf, actions, legal, top=5, temperature=0.9)
+  grad, = torch.autograd.grad([r.logprob, r.entropy, r.top_logprob], leaf, [gl, gh, gt])
+  loss, h, both = torch.empty(n, device="cuda"), torch.empty(n, device="cuda"), torch.empty_like(x)
+  policy.distill_into(x, w, loss, h, ids, legal, "weights", 0.9, weight, both)
+  alone, _ = policy.distill(leaf, w, ids, legal, temperature=0.9)
+  again, = torch.autograd.grad((alone * weight).sum(), leaf)
+  with torch.device("cuda"):
+    want, tol = ref.logprobs(x, actions, legal, 5, 0.9)
+    for key in ("logprob", "entropy", "top_logprob"):
+      held_there(getattr(r, key), want[key], tol[key], key)
+    assert torch.equal(r.top_action, want["top_action"])
+    want, tol = ref.logprobs_grad(x, actions, legal, 0.9, gl, gh, r.top_action, gt)
+    held_there(grad, want, tol + ref.rounding(x.dtype, want), "grad")
+    want, tol = ref.distill(x, w, ids, legal, "weights", 0.9, weight)
+    held_there(loss, want["loss"], tol["loss"], "loss")
+    held_there(alone, want["loss"], tol["loss"], "loss alone")
+    held_there(h, want["entropy"], tol["entropy"], "target entropy")
+    for got in (both, again):
+      held_there(got, want["grad"], tol["grad"] + ref.rounding(x.dtype, want["grad"]), "grad")
+
+
+@gpu
+@pytest.mark.parametrize("n,v,dtype", [(2300, 33001, "f32"), (2100, 70002, "bf16"),
+                                       (2100, 70001, "f16"), (1500, 60000, "f32")])
+def test_gpu_more_logits_than_the_cache(require_gpu, n, v, dtype):
+  """Batches of more than 256 MiB equal their halves, bit for bit."""
+  from os_amd import policy
+  g = torch.Generator(device="cuda").manual_seed(v)
+  f = dict(device="cuda", generator=g)
+  x = torch.randn(n, v, **f).to(TYPES[dtype])
+  actions = torch.randint(0, v, (n,), **f)
+  ids = torch.randint(0, v, (n, 64), **f)
+  w = torch.rand(n, 64, **f)
+  gl = torch.randn(n, **f)
+
+  def run(rows):
+    leaf = x[rows].requires_grad_()
+    r = policy.logprobs(leaf, actions[rows], top=7)
+    grad, = torch.autograd.grad([r.logprob, r.entropy], leaf, [gl[rows], gl[rows]])
+    m = len(leaf)
+    loss, h, both = (torch.empty(m, device="cuda"), torch.empty(m, device="cuda"),
+                     torch.empty(m, v, dtype=x.dtype, device="cuda"))
+    policy.distill_into(x[rows], w[rows], loss, h, ids[rows], weight=gl[rows], grad=both)
+    alone, _ = policy.distill(leaf, w[rows], ids[rows])
+    again, = torch.autograd.grad(alone, leaf, gl[rows])
+    return [r.logprob, r.entropy, r.top_action, r.top_logprob, grad, loss, h, both, alone, again]
+  half = n // 2
+  # (both above a thousand rows or both below: the same kernels)
+  whole, parts = run(slice(0, n)), [run(slice(0, half)), run(slice(half, n))]
+  if half >= 1024:
+    for i, p in enumerate(whole):
+      assert torch.equal(p, torch.cat([q[i] for q in parts])), i
+  last = slice(n - 40, n)
+  with torch.device("cuda"):
+    want, tol = ref.logprobs(x[last], actions[last], None, 7)
+    held_there(whole[0][last], want["logprob"], tol["logprob"], "logprob")
+    assert torch.equal(whole[2][last], want["top_action"])
+    want, tol = ref.logprobs_grad(x[last], actions[last], None, 1.0, gl[last], gl[last])
+    held_there(whole[4][last], want, tol + ref.rounding(x.dtype, want), "grad")
+    want, tol = ref.distill(x[last], w[last], ids[last], weight=gl[last])
+    held_there(whole[5][last], want["loss"], tol["loss"], "loss")
+    for i in (7, 9):
+      held_there(whole[i][last], want["grad"], tol["grad"] + ref.rounding(x.dtype, want["grad"]),
+                 "grad")
+
+
+@gpu
+@pytest.mark.parametrize("t", [1.0, 0.25, 3.0])
+@pytest.mark.parametrize("v", [50, 900, 2500, 20011, 150001])
+def test_gpu_common_offsets(require_gpu, v, t):
+  """Rows far from zero on either side of where the scaled maximum has no
+  fraction left (2^24), actions a few units below the maximum included."""
+  edge = 2.0 ** 24 / math.log2(math.e) * t
+  tops = [s * (edge + d) for s in (-1.0, 1.0) for d in (-1000.0, -150.0, -4.0, -1.0, 1.0, 40.0)]
+  tops += [1e8, -1e8, 1e30, -1e30]
+  g = torch.Generator().manual_seed(v)
+  logits = torch.stack([torch.tensor(m) - torch.randint(1, 30, (v,), generator=g) for m in tops])
+  logits[:, v // 3] = torch.tensor(tops)
+  n = len(tops)
+  actions = torch.randint(0, v, (n,), generator=g)
+  check_logprobs(logits, None, actions, 3, t)
+  target, ids = make_target(n, v, 6, None, "weights")
+  check_distill(logits, None, target, ids, "weights", t)
+  gl, gh = torch.randn(n, generator=g), torch.randn(n, generator=g)
+  from os_amd import policy
+  leaf = logits.cuda().requires_grad_()
+  r = policy.logprobs(leaf, actions.cuda(), temperature=t)
+  grad, = torch.autograd.grad([r.logprob, r.entropy], leaf, [gl.cuda(), gh.cuda()])
+  want, tol = ref.logprobs_grad(logits, actions, None, t, gl, gh)
+  close(grad, want, tol + ref.rounding(grad.dtype, want), "grad")
+
+
+@gpu
+@pytest.mark.parametrize("v,k", [(40, 1024), (700, 1024), (2047, 700), (20011, 1024)])
+def test_gpu_distill_long_lists_with_repeats(require_gpu, v, k):
+  n = 7
+  logits, _, _ = make(n, v, "f32", False, seed=9)
+  g = torch.Generator().manual_seed(v + k)
+  ids = torch.randint(-1, max(2, v // 2), (n, k), generator=g)
+  w = torch.rand(n, k, generator=g)
+  check_distill(logits, None, w, ids, "weights", 1.0, torch.randn(n, generator=g))
+  check_distill(logits, None, (w * 5).to(torch.float16), ids, "logits", 0.8, None, wide=False)
+
+
 @gpu
 def test_gpu_gradient_against_differences(require_gpu):
   """The kernels' own losses at x +- h: central differences with h = 2^-5 are
