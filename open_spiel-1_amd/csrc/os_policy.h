@@ -148,6 +148,7 @@ template <class T>
 constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // elements of a 16-byte chunk
 
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
 using f32x2 = __attribute__((ext_vector_type(2))) float;
 
 __device__ __forceinline__ float get(const float* p, int64_t i) { return p[i]; }
@@ -178,22 +179,29 @@ struct __attribute__((packed, aligned(1))) MaskWord {
     return (w[j / 4] & (0xFFu << (8 * (j % 4)))) != 0;
   }
 };
+template <>
+struct __attribute__((packed, aligned(1))) MaskWord<2> {
+  uint16_t w;
+  __device__ __forceinline__ bool allows(int j) const { return (w & (0xFFu << (8 * j))) != 0; }
+};
 
-template <class T>
-__device__ __forceinline__ void unpack(u32x4 r, float (&x)[kPer<T>]) {
+// A chunk of kE elements: W is u32x4, or u32x2 (k_wave).
+template <class T, class W, int kE>
+__device__ __forceinline__ void unpack(W r, float (&x)[kE]) {
+  static_assert(sizeof(W) == kE * sizeof(T));
   if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(r[j]);
+    for (int j = 0; j < kE; ++j) x[j] = __uint_as_float(r[j]);
   } else if constexpr (std::is_same_v<T, __bf16>) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kE / 2; ++j) {
       x[2 * j] = __uint_as_float(r[j] << 16);
       x[2 * j + 1] = __uint_as_float(r[j] & 0xFFFF0000u);
     }
   } else {
     using h2 = __attribute__((ext_vector_type(2))) _Float16;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kE / 2; ++j) {
       const h2 h = __builtin_bit_cast(h2, static_cast<uint32_t>(r[j]));
       x[2 * j] = static_cast<float>(h[0]);
       x[2 * j + 1] = static_cast<float>(h[1]);
@@ -201,16 +209,17 @@ __device__ __forceinline__ void unpack(u32x4 r, float (&x)[kPer<T>]) {
   }
 }
 // Round to nearest even, once.
-template <class T>
-__device__ __forceinline__ u32x4 pack(const float (&x)[kPer<T>]) {
-  u32x4 r;
+template <class T, class W, int kE>
+__device__ __forceinline__ W pack(const float (&x)[kE]) {
+  static_assert(sizeof(W) == kE * sizeof(T));
+  W r;
   if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = __float_as_uint(x[j]);
+    for (int j = 0; j < kE; ++j) r[j] = __float_as_uint(x[j]);
   } else {
     using h2 = __attribute__((ext_vector_type(2))) T;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kE / 2; ++j) {
       const f32x2 f = {x[2 * j], x[2 * j + 1]};
       r[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, h2));
     }
@@ -780,9 +789,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
 #pragma unroll
       for (int j = 0; j < kE; ++j)
         if (oc + j < o) x[j] = neg_inf();
-      if constexpr (kSums && kSecond && !kMask) raw[t] = pack<T>(x);
+      if constexpr (kSums && kSecond && !kMask) raw[t] = pack<T, u32x4>(x);
     }
-    if constexpr (kSums && kSecond && kMask) raw[t] = pack<T>(x);
+    if constexpr (kSums && kSecond && kMask) raw[t] = pack<T, u32x4>(x);
   };
   // The same again, once values() has left the exclusions in the registers.
   auto again = [&](int t, float (&x)[kE], int ln) {
@@ -1245,7 +1254,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
           }
           if (o + kE <= ln) {
             const uint32_t bytes = static_cast<uint32_t>(o) * static_cast<uint32_t>(sizeof(T));
-            store_at<kStream>(reinterpret_cast<T*>(reinterpret_cast<char*>(gb) + bytes), pack<T>(y));
+            store_at<kStream>(reinterpret_cast<T*>(reinterpret_cast<char*>(gb) + bytes), pack<T, u32x4>(y));
           } else if (o < ln) {
 #pragma unroll
             for (int j = 0; j < kE; ++j)
@@ -1318,21 +1327,27 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
 
 // ---- rows of up to four chunks a lane: a wave each ----
 
-// kC chunks a lane, the values in registers as floats; the next row's chunks
-// are under way while a row is worked on.  No barrier is needed: what goes
+// kC chunks of 8 or 16 bytes (W) a lane, the values in registers as floats; the
+// next row's chunks are under way while a row is worked on.  Rows take the
+// smallest kernel that holds them, so only the last chunk is ever short: the
+// arithmetic, not the memory, is what a row costs here (65536 x 768 masked bf16,
+// top 8: two chunks of 16 bytes 60 us, three of 8 bytes 56 us).  No barrier is needed: what goes
 // through LDS stays within the wave, whose accesses are in order (fence() keeps
 // the compiler to it).
 // Waves a SIMD that the registers must leave room for (left alone, the compiler
 // keeps every address it could compute again): latency is hidden by waves here.
 template <bool kMask, int kX, int kOp>
 constexpr int kWaveRoom = kOp == kLogprobs || kOp == kLogprobsTop ? (kX <= 16 ? 6 : 4)
-                          : kOp == kDistill                       ? (kX <= 8 ? 6 : kX == 16 ? 5 : 4)
+                          : kOp == kDistill                       ? (kX <= 8 ? 6 : kX <= 16 ? 5 : 4)
                           : kX <= 8                               ? (kMask ? 4 : 5)
-                          : kX == 16                              ? 4
+                          : kX <= 16                              ? 4
                                                                   : 2;
-template <class T, bool kMask, int kC, int kOp>
-__global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_wave(Rows a, ArgsOf<kOp> g) {
-  constexpr int kE = kPer<T>, kX = kC * kE;
+template <class T, class W, int kC>
+constexpr int kWaveEach = kC * static_cast<int>(sizeof(W) / sizeof(T));  // elements a lane
+template <class T, bool kMask, class W, int kC, int kOp>
+__global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) void k_wave(
+    Rows a, ArgsOf<kOp> g) {
+  constexpr int kE = static_cast<int>(sizeof(W) / sizeof(T)), kX = kC * kE;
   constexpr bool kSums = kOp != kLogprobsGrad && kOp != kDistillGrad;
   constexpr bool kGrad = kOp == kLogprobsGrad || kOp == kDistillGrad || kOp == kDistillFused;
   constexpr bool kLp = kOp == kLogprobs || kOp == kLogprobsTop;
@@ -1348,7 +1363,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_w
   const int last = a.v - kE;
   const auto fence = [] { __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront"); };
 
-  u32x4 raw[kC];
+  W raw[kC];
   Word mk[kMask ? kC : 1];
   const auto load = [&](int64_t r) {
     const T* const x = static_cast<const T*>(a.x) + r * a.ld;
@@ -1356,7 +1371,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_w
 #pragma unroll
     for (int t = 0; t < kC; ++t) {
       const int oc = min((t * 64 + lane) * kE, last);
-      raw[t] = load_at<false, T, u32x4>(x + oc);
+      raw[t] = load_at<false, T, W>(x + oc);
       if constexpr (kMask) mk[t] = *reinterpret_cast<const Word*>(legal + oc);
     }
   };
@@ -1365,10 +1380,8 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_w
   const int edge = a.v / kE * kE, shift = (kE - a.v % kE) % kE;
   const auto slot = [&](int id) { return id + (id >= edge ? shift : 0); };
 
-  // How many elements of a chunk come before its own start (see load()).
-  int drop[kC - kC / 2];
-#pragma unroll
-  for (int t = kC / 2; t < kC; ++t) drop[t - kC / 2] = (t * 64 + lane) * kE - min((t * 64 + lane) * kE, last);
+  // How many elements of the last chunk come before its own start (see load()).
+  const int drop = ((kC - 1) * 64 + lane) * kE - min(((kC - 1) * 64 + lane) * kE, last);
 
   RowValues<kOp> next = RowValues<kOp>::at(g, blockIdx.x);
   load(blockIdx.x);
@@ -1388,10 +1401,10 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_w
         for (int j = 0; j < kE; ++j)
           if (!mk[t].allows(j)) x[t * kE + j] = neg_inf();
       }
-      if (t >= kC / 2) {  // (the first half is full: fewer chunks would do else)
+      if (t == kC - 1) {
 #pragma unroll
         for (int j = 0; j < kE; ++j)
-          if (j < drop[t - kC / 2]) x[t * kE + j] = neg_inf();
+          if (j < drop) x[t * kE + j] = neg_inf();
       }
     }
     // -- what else the row needs from memory, ahead of the next row's loads --
@@ -1537,8 +1550,8 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_w
     float f0 = 0.0f, f1 = 0.0f;
     const auto clear = [&] {
 #pragma unroll
-      for (int t = 0; t < kX / 4; ++t)
-        *reinterpret_cast<u32x4*>(row + (t * 64 + lane) * 4) = u32x4{0, 0, 0, 0};
+      for (int t = 0; t < kX / 2; ++t)
+        *reinterpret_cast<u32x2*>(row + (t * 64 + lane) * 2) = u32x2{0, 0};
     };
     [[maybe_unused]] int* const tag = reinterpret_cast<int*>(row);
     if constexpr (kTarget) {
@@ -1717,8 +1730,8 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kC * kPer<T>, kOp>)) void k_w
           for (int j = 0; j < kE; ++j) y[j] += dn.template any<kLog>(x[t * kE + j]);
         }
         const int o = (t * 64 + me) * kE;
-        if (t < kC / 2 || o + kE <= a.v) {
-          store_at<false>(gb + o, pack<T>(y));
+        if (t < kC - 1 || o + kE <= a.v) {
+          store_at<false>(gb + o, pack<T, W>(y));
         } else if (o < a.v) {
 #pragma unroll
           for (int j = 0; j < kE; ++j)
@@ -2051,17 +2064,17 @@ __global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
 // ---- launches (one unit a type) ----
 
 // Static LDS, bytes (rounded up).
-template <class T, int kC, int kOp>
+template <class T, class W, int kC, int kOp>
 constexpr int kWaveLds = kOp == kLogprobsTop ? kWaveCandidates * 16
                          : kOp == kLogprobs  ? 0
-                                             : 64 * kC * kPer<T> * 4;
+                                             : 64 * kWaveEach<T, W, kC> * 4;
 constexpr int kRowsLds = 8 * 1024;
 
 struct Launch {
   Rows a;
   Parts pt;
   int waves;       // 0: k_tiny
-  int wave;        // chunks a lane of k_wave (1, 2 or 4), 0: k_rows
+  int wave;        // k_wave: what it holds in units of 512 bytes, 0: k_rows
   int chunks;      // a lane of k_rows
   bool streamed;   // k_rows: see kStream
   unsigned lds;    // dynamic, bytes

@@ -27,7 +27,7 @@ static_assert(OS_AZ_NO_WORKSPACE_ACTIONS * 4 <= kWholeRow);
 
 struct Plan {
   int waves;  // 0: k_tiny
-  int wave;   // chunks a lane of k_wave, 0: k_rows
+  int wave;   // k_wave: what it holds in units of 512 bytes, 0: k_rows
   int chunks;  // a lane of k_rows
   bool streamed;  // k_rows does not ask the caches to keep the logits
   Parts pt;
@@ -53,7 +53,8 @@ bool short_rows(const Rows& a, int size, Plan* p) {
   p->pt = Parts{1, a.v};
   if (a.v <= kTinyMax) return true;
   p->waves = 1;
-  p->wave = bytes <= kKib ? 1 : bytes <= 2 * kKib ? 2 : 4;
+  const int units = static_cast<int>(up(bytes, 512));
+  p->wave = units <= 4 ? units : units <= 6 ? 6 : 8;
   return true;
 }
 

@@ -40,20 +40,27 @@ void launch_rows(const Launch& c, const G& g) {
     return;
   }
   if (c.wave != 0) {
-    const auto go = [&](auto mask, auto chunks) {
+    const auto go = [&](auto mask, auto chunk, auto chunks) {
+      using W = decltype(chunk);
       constexpr bool kMask = decltype(mask)::value;
       constexpr int kC = decltype(chunks)::value;
-      constexpr auto kernel = &k_wave<T, kMask, kC, kOp>;
-      hipLaunchKernelGGL(kernel, row_grid(c, waves_per_simd<kernel>(), kWaveLds<T, kC, kOp>),
+      constexpr auto kernel = &k_wave<T, kMask, W, kC, kOp>;
+      hipLaunchKernelGGL(kernel, row_grid(c, waves_per_simd<kernel>(), kWaveLds<T, W, kC, kOp>),
                          dim3(64), 0, c.stream, c.a, g);
     };
     constexpr std::integral_constant<int, 1> one;
     constexpr std::integral_constant<int, 2> two;
+    constexpr std::integral_constant<int, 3> three;
     constexpr std::integral_constant<int, 4> four;
     const auto by_chunks = [&](auto mask) {
-      if (c.wave == one) go(mask, one);
-      else if (c.wave == two) go(mask, two);
-      else go(mask, four);
+      switch (c.wave) {
+        case 1: return go(mask, u32x2{}, one);
+        case 2: return go(mask, u32x4{}, one);
+        case 3: return go(mask, u32x2{}, three);
+        case 4: return go(mask, u32x4{}, two);
+        case 6: return go(mask, u32x4{}, three);
+        default: return go(mask, u32x4{}, four);
+      }
     };
     if (c.a.legal != nullptr) by_chunks(std::true_type{});
     else by_chunks(std::false_type{});
