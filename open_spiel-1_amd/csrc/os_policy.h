@@ -47,7 +47,7 @@ constexpr int kTinyMax = 64;       // rows of up to this many actions: 16 lanes 
 constexpr int kMaxWaves = 16;
 constexpr int kMaxSplit = 64;      // parts of a row
 constexpr int kCandidates = 512;   // top actions: LDS list
-constexpr int kWaveCandidates = 256;  // of a wave alone (a multiple of 64)
+constexpr int kWaveCandidates = 192;  // of a wave alone (a multiple of 64)
 constexpr int kFewChunks = 4;      // chunks a lane: the most of k_wave, the least of k_rows,
 constexpr int kMidChunks = 8;      // its most with a mask
 constexpr int kChunks = 16;        // and without
@@ -176,7 +176,7 @@ template <int kE>
 struct __attribute__((packed, aligned(1))) MaskWord {
   uint32_t w[kE / 4];
   __device__ __forceinline__ bool allows(int j) const {
-    return (w[j / 4] & (0xFFu << (8 * (j % 4)))) != 0;
+    return static_cast<uint8_t>(w[j / 4] >> (8 * (j % 4))) != 0;
   }
 };
 template <>
@@ -562,28 +562,29 @@ __device__ __forceinline__ uint64_t fold64_max(uint64_t v) {
 }
 // One of the lanes' values with at least k of them at or above it, and usually
 // few more (-inf where fewer than k lanes hold any): a bound of the k-th largest
-// element from below.  Bisection between the least and the largest, counting
-// with ballots on the scalar unit: six steps or so, where ranking every lane
-// against every other takes 192 vector operations.
-// `most` is the lanes' largest; kExact: the bound is a lane's value.
-template <bool kExact>
+// element from below.  Bisection between the least and the largest (`most`) over
+// 2^16 steps, counting with ballots on the scalar unit: six rounds or so of one
+// vector operation, where ranking every lane against every other takes 192.
 __device__ __forceinline__ float kth_bound(float v, float most, int k) {
   if (k == 1) return most;
   const float inf = __builtin_huge_valf();
   const bool any = v > neg_inf();
   if (__builtin_popcountll(__ballot(any)) < k) return neg_inf();
-  float lo = -fold64(any ? -v : -inf, Max{});
-  float hi = most;
+  // (halves: the difference of two finite values is finite)
+  const float least = -0.5f * fold64(any ? -v : -inf, Max{});
+  const float scale = 65535.0f * __builtin_amdgcn_rcpf(fmaf(most, 0.5f, -least));
+  const int q = any ? static_cast<int>(fminf(fmaf(v, 0.5f, -least) * scale, 65535.0f)) : -1;
   const int enough = k + (k >> 2) + 3;
-  for (int step = 0; step < 24; ++step) {
-    const float mid = fmaf(lo, 0.5f, hi * 0.5f);
-    if (!(mid > lo && mid < hi)) break;
-    const int n = __builtin_popcountll(__ballot(v >= mid));
+  int lo = 0, hi = 65536;
+#pragma unroll 1
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    const int n = __builtin_popcountll(__ballot(q >= mid));
     if (n >= k) lo = mid;
     else hi = mid;
     if (n >= k && n <= enough) break;
   }
-  return kExact ? -fold64(v >= lo ? -v : -inf, Max{}) : lo;
+  return -fold64(q >= lo ? -v : -inf, Max{});
 }
 
 // The k-th largest (k >= 1) of one key a lane.
@@ -1037,7 +1038,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
           const uint64_t key = nw == 1 ? lane_key : top_lds.group[lane];
           const float v = key == 0 ? neg_inf() : key_value(key);
           const int at = key == 0 ? 0x7FFFFFFF : static_cast<int>(key_index(key));
-          const float tv = kth_bound<true>(v, m, g.top);
+          const float tv = kth_bound(v, m, g.top);
           // of those at the bound, as many as `top` still needs, the first
           const uint64_t tied = __ballot(v == tv && key != 0);
           const int need = g.top - __builtin_popcountll(__ballot(v > tv));
@@ -1337,7 +1338,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
 // Waves a SIMD that the registers must leave room for (left alone, the compiler
 // keeps every address it could compute again): latency is hidden by waves here.
 template <bool kMask, int kX, int kOp>
-constexpr int kWaveRoom = kOp == kLogprobs || kOp == kLogprobsTop ? (kX <= 16 ? 6 : 4)
+constexpr int kWaveRoom = kOp == kLogprobs || kOp == kLogprobsTop ? (kX <= 12 ? 8 : kX <= 16 ? 6 : 4)
                           : kOp == kDistill                       ? (kX <= 8 ? 6 : kX <= 16 ? 5 : 4)
                           : kX <= 8                               ? (kMask ? 4 : 5)
                           : kX <= 16                              ? 4
@@ -1357,7 +1358,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
   // The row's values, then its listed weights: chunk (t, lane) at
   // (t * 64 + lane) * kE, the row's last actions where their chunk has them.
   __shared__ __attribute__((aligned(16))) float row[kTarget || kGrad ? 64 * kX : 1];
-  __shared__ Found cand[kOp == kLogprobsTop ? kWaveCandidates : 1];
+  __shared__ Found cand[kOp == kLogprobsTop ? kWaveCandidates + 64 : 1];
   __shared__ uint64_t keys[kOp == kLogprobsTop ? kWaveCandidates : 1];
   const int lane = threadIdx.x;
   const int last = a.v - kE;
@@ -1486,7 +1487,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
         g.top_logprob[r * g.top + rank] =
             odd ? l : key == 0 ? neg_inf() : log_p(a, key_value(key), m, l);
       };
-      const float bound = fmaxf(kth_bound<false>(lane_max, m, g.top), kLowest);
+      const float bound = fmaxf(kth_bound(lane_max, m, g.top), kLowest);
       int found = 0;
       renew(me);
       if (!odd) {
@@ -1501,7 +1502,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
               const int at = __builtin_amdgcn_mbcnt_hi(
                   static_cast<uint32_t>(hit >> 32),
                   __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hit), found));
-              if (in && at < kWaveCandidates) cand[at] = Found{x[t * kE + j], oc + j};
+              if (in && found <= kWaveCandidates) cand[at] = Found{x[t * kE + j], oc + j};
               found += __builtin_popcountll(hit);
             }
           }
@@ -2065,7 +2066,7 @@ __global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
 
 // Static LDS, bytes (rounded up).
 template <class T, class W, int kC, int kOp>
-constexpr int kWaveLds = kOp == kLogprobsTop ? kWaveCandidates * 16
+constexpr int kWaveLds = kOp == kLogprobsTop ? kWaveCandidates * 16 + 512
                          : kOp == kLogprobs  ? 0
                                              : 64 * kWaveEach<T, W, kC> * 4;
 constexpr int kRowsLds = 8 * 1024;
