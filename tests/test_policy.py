@@ -810,6 +810,30 @@ def test_gpu_search_then_train(require_gpu, game):
 
 
 @gpu
+def test_gpu_documented_training_step(require_gpu):
+  """INTEGRATION.md's block runs as written and reaches the model's weights."""
+  import os
+  import re
+  doc = open(os.path.join(os.path.dirname(__file__), "..", "INTEGRATION.md")).read()
+  block, = [b for b in re.findall(r"```python\n(.*?)```", doc, flags=re.S)
+            if "policy.search_targets" in b]
+  n, a = 20, 9
+  nchild = np.array([r % 4 for r in range(n)], np.int32)
+  model = torch.nn.Linear(5, a + 1).cuda()
+  env = dict(model=model, num_actions=a, obs=torch.randn(n, 5, device="cuda"),
+             legal=torch.ones(n, a, dtype=torch.uint8, device="cuda"),
+             moves=torch.arange(n, device="cuda") % a - 1,
+             out=dict(nchild=nchild, child_action=np.tile(np.arange(a, dtype=np.int32), (n, 1)),
+                      child_n=np.ones((n, a), np.int32)))
+  exec(block, env)
+  want, tol = ref.distill(env["logits"].detach().cpu(), env["counts"].cpu(), env["ids"].cpu())
+  close(env["loss"], want["loss"], tol["loss"], "loss")
+  assert env["r"].top_action.shape == (n, 3)
+  assert bool(torch.isfinite(model.weight.grad).all()) and bool((model.weight.grad[:a] != 0).any())
+  assert bool((model.weight.grad[a] == 0).all())
+
+
+@gpu
 def test_gpu_selfplay_visits_as_target(require_gpu):
   """Engine.selfplay's dense int32 visits, padded moves among them."""
   from os_amd import policy
