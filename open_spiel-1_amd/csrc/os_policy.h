@@ -451,8 +451,9 @@ __device__ __forceinline__ void target_entries(const Target& t, int64_t r, int f
   });
 }
 // The same in two halves, as they lie in memory in between: load() issues every
-// load and finish() is the first to wait for one.  (Held across a row by k_rows;
-// k_wave's six entries a lane would spill as this form.)
+// load and finish() is the first to wait for one.  (Held across a row by k_rows.
+// k_wave's six entries a lane, held across the sums in this form, spill: 16384 x
+// 362 visit counts 33 -> 43 us.)
 template <int kCount>
 struct RawEntries {
   int64_t id[kCount];
