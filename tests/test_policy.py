@@ -427,6 +427,7 @@ def held_there(got, want, tol, what):
 
 @gpu
 @pytest.mark.parametrize("n,v,k,dtype,masked", [
+    (1200, 1500, 70, "f32", False), (2600, 3001, 200, "bf16", True), (1100, 2047, 33, "f32", True),
     (1200, 2500, 1024, "f32", False), (1200, 2500, 600, "f32", True), (2600, 4099, 70, "f16", True),
     (2600, 4099, 70, "bf16", False), (1100, 9001, 70, "f32", False), (1100, 9001, 300, "bf16", True),
     (1030, 40000, 70, "bf16", False), (1030, 40001, 70, "f32", True), (1030, 70001, 9, "f32", False)])
@@ -546,6 +547,19 @@ def test_gpu_common_offsets(require_gpu, v, t):
   want, tol = ref.logprobs_grad(logits, actions, None, t, gl, gh)
   close(grad, want, tol + ref.rounding(grad.dtype, want), "grad")
 
+
+@gpu
+@pytest.mark.parametrize("n,v,dtype,masked", [(2, 1 << 21, "f32", False), (1, (1 << 21) - 1, "f32", True),
+                                              (3, (1 << 21) - 63, "bf16", True),
+                                              (70, (1 << 20) + 1, "f16", False)])
+def test_gpu_largest_rows(require_gpu, n, v, dtype, masked):
+  logits, legal, actions = make(n, v, dtype, masked, seed=2)
+  check_logprobs(logits, legal, actions, 64)
+  target, ids = make_target(n, v, 64, legal, "weights")
+  ids[:, -1] = torch.where(ids[:, 0] >= 0, v - 1, -1)
+  if masked:
+    legal[:, v - 1] = torch.where(ids[:, 0] >= 0, 1, 0).to(torch.uint8)
+  check_distill(logits, legal, target, ids, "weights")
 
 @gpu
 @pytest.mark.parametrize("v,k", [(40, 1024), (700, 1024), (2047, 700), (20011, 1024)])
