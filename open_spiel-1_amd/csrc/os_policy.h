@@ -51,8 +51,9 @@ constexpr int kMaxWaves = 16;
 constexpr int kMaxSplit = 64;      // parts of a row
 constexpr int kCandidates = 512;   // top actions: LDS list
 constexpr int kWaveCandidates = 192;  // of a wave alone (a multiple of 64)
-constexpr int kFewChunks = 4;      // chunks a lane: the most of k_wave, the least of k_rows,
-constexpr int kMidChunks = 8;      // its most with a mask
+constexpr int kWaveMax = 2048;     // of up to this many: a wave each, 32 actions a lane
+constexpr int kFewChunks = 4;      // chunks a lane of k_rows: the least,
+constexpr int kMidChunks = 8;      // the most with a mask
 constexpr int kChunks = 16;        // and without
 
 struct Rows {
@@ -1330,7 +1331,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
   }
 }
 
-// ---- rows of up to four chunks a lane: a wave each ----
+// ---- rows of up to kWaveMax actions: a wave each ----
 
 // kC chunks of 8 or 16 bytes (W) a lane, the values in registers as floats; the
 // next row's chunks are under way while a row is worked on.  No barrier is
@@ -1339,8 +1340,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
 // waits for here, 30 operations an element with the mask and the top actions
 // (65536 x 768 masked bf16, top 8: 52 us, units 73% busy; 32 us is the
 // memory's share), so rows take the smallest kernel that holds them and only the
-// last chunk is ever short (the same in two chunks of 16 bytes rather than three
-// of 8: 4 us more).
+// last chunk is ever short, of six and eight the last two (the same in two chunks
+// of 16 bytes rather than three of 8: 4 us more).  Against a workgroup of k_rows
+// it saves the barriers: 44739 x 1500 f32, top 8: 99 -> 54 us, loss and gradient:
+// 152 -> 115 us.
 // Waves a SIMD that the registers must leave room for (left alone, the compiler
 // keeps every address it could compute again): what the dependent steps of a row
 // leave idle, other rows fill (8 rather than 7 at that size: 57 -> 53 us).
@@ -1388,8 +1391,13 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
   const int edge = a.v / kE * kE, shift = (kE - a.v % kE) % kE;
   const auto slot = [&](int id) { return id + (id >= edge ? shift : 0); };
 
-  // How many elements of the last chunk come before its own start (see load()).
-  const int drop = ((kC - 1) * 64 + lane) * kE - min(((kC - 1) * 64 + lane) * kE, last);
+  // Chunks that every row of this kernel fills (a smaller kernel takes the rest),
+  // and how many elements of the others come before their own start (see load()).
+  constexpr int kFull = kC - (kC > 4 ? 2 : 1);
+  int drop[kC - kFull];
+#pragma unroll
+  for (int t = kFull; t < kC; ++t)
+    drop[t - kFull] = (t * 64 + lane) * kE - min((t * 64 + lane) * kE, last);
 
   RowValues<kOp> next = RowValues<kOp>::at(g, blockIdx.x);
   load(blockIdx.x);
@@ -1409,10 +1417,10 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
         for (int j = 0; j < kE; ++j)
           if (!mk[t].allows(j)) x[t * kE + j] = neg_inf();
       }
-      if (t == kC - 1) {
+      if (t >= kFull) {
 #pragma unroll
         for (int j = 0; j < kE; ++j)
-          if (j < drop) x[t * kE + j] = neg_inf();
+          if (j < drop[t - kFull]) x[t * kE + j] = neg_inf();
       }
     }
     // -- what else the row needs from memory, ahead of the next row's loads --
@@ -1738,7 +1746,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
           for (int j = 0; j < kE; ++j) y[j] += dn.template any<kLog>(x[t * kE + j]);
         }
         const int o = (t * 64 + me) * kE;
-        if (t < kC - 1 || o + kE <= a.v) {
+        if (t < kFull || o + kE <= a.v) {
           store_at<false>(gb + o, pack<T, W>(y));
         } else if (o < a.v) {
 #pragma unroll

@@ -18,7 +18,6 @@ using namespace osp;
 constexpr int kCus = 256;
 constexpr int64_t kKib = 1024;
 constexpr int64_t kLastLevelCache = int64_t{256} << 20;
-constexpr int64_t kWaveFew = kFewChunks * kKib;  // bytes a wave holds: 64 lanes x 16 a chunk
 // (sums_plan leaves rows that fit a workgroup whole, masked or not)
 constexpr int64_t kWholeRow = kMaxWaves * kMidChunks * kKib;
 static_assert(OS_AZ_NO_WORKSPACE_ACTIONS * 4 <= kWholeRow);
@@ -46,18 +45,19 @@ Parts split(int32_t v, int64_t parts) {
   return p;
 }
 
-// Rows of at most four chunks a lane: 16 lanes or a wave each.
+// Rows of up to kWaveMax actions: 16 lanes or a wave each.
 bool short_rows(const Rows& a, int size, Plan* p) {
   const int64_t bytes = int64_t{a.v} * size;
-  if (bytes > kWaveFew && a.v > kTinyMax) return false;
+  if (a.v > kWaveMax) return false;
   p->pt = Parts{1, a.v};
   if (a.v <= kTinyMax) return true;
   p->waves = 1;
   const int units = static_cast<int>(up(bytes, 512));
-  p->wave = units <= 4 ? units : units <= 6 ? 6 : 8;
+  p->wave = units <= 4 ? units : units <= 6 ? 6 : units <= 8 ? 8 : units <= 12 ? 12 : 16;
   return true;
 }
 
+// Bytes a wave of k_rows holds: 64 lanes x 16 a chunk.
 int64_t wave_bytes(const Rows& a) { return (a.legal ? kMidChunks : kChunks) * kKib; }
 
 // Chunks a lane and waves for `bytes` a workgroup: with `wide` as many waves as
@@ -66,7 +66,7 @@ int64_t wave_bytes(const Rows& a) { return (a.legal ? kMidChunks : kChunks) * kK
 // listed actions are read again and 16 would crowd them out of the cache).
 void fit(const Rows& a, int size, int64_t bytes, bool wide, Plan* p) {
   const int64_t most = wave_bytes(a);
-  if (wide && bytes <= kMaxWaves * kWaveFew) p->chunks = kFewChunks;
+  if (wide && bytes <= kMaxWaves * kFewChunks * kKib) p->chunks = kFewChunks;
   else if (bytes <= (wide ? kMaxWaves * kMidChunks : kChunks) * kKib || most == kMidChunks * kKib)
     p->chunks = kMidChunks;
   else p->chunks = kChunks;

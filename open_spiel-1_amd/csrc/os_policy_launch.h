@@ -52,6 +52,8 @@ void launch_rows(const Launch& c, const G& g) {
     constexpr std::integral_constant<int, 2> two;
     constexpr std::integral_constant<int, 3> three;
     constexpr std::integral_constant<int, 4> four;
+    [[maybe_unused]] constexpr std::integral_constant<int, 6> six;
+    [[maybe_unused]] constexpr std::integral_constant<int, 8> eight;
     const auto by_chunks = [&](auto mask) {
       switch (c.wave) {
         case 1: return go(mask, u32x2{}, one);
@@ -59,7 +61,12 @@ void launch_rows(const Launch& c, const G& g) {
         case 3: return go(mask, u32x2{}, three);
         case 4: return go(mask, u32x4{}, two);
         case 6: return go(mask, u32x4{}, three);
-        default: return go(mask, u32x4{}, four);
+        case 8: return go(mask, u32x4{}, four);
+        default:
+          if constexpr (sizeof(T) == 4) {
+            if (c.wave == 12) go(mask, u32x4{}, six);
+            else go(mask, u32x4{}, eight);
+          }
       }
     };
     if (c.a.legal != nullptr) by_chunks(std::true_type{});
