@@ -61,21 +61,23 @@ bool short_rows(const Rows& a, int size, Plan* p) {
 int64_t wave_bytes(const Rows& a) { return (a.legal ? kMidChunks : kChunks) * kKib; }
 
 // Chunks a lane and waves for `bytes` a workgroup: with `wide` as many waves as
-// a workgroup has (few rows: each is over sooner), else as few as the registers
-// allow (more rows at once, fewer waves to join; 8 chunks up to 16 KiB, where
-// listed actions are read again and 16 would crowd them out of the cache).
+// a workgroup has (few rows: each is over sooner), else eight chunks as long as
+// they do (4194 x 16000 f32, loss and gradient: 146 us in four, 123 in eight, 136
+// in sixteen).  Logits beyond the last-level cache want fewer, longer waves and
+// no place in the cache, once rows fill them (1 GiB of f32, loss and gradient:
+// rows of 32768 445 us in eight, 425 in sixteen; rows of 4100 515 and 733).
 void fit(const Rows& a, int size, int64_t bytes, bool wide, Plan* p) {
-  const int64_t most = wave_bytes(a);
+  const bool cached = a.n * a.v * size <= kLastLevelCache;
   if (wide && bytes <= kMaxWaves * kFewChunks * kKib) p->chunks = kFewChunks;
-  else if (bytes <= (wide ? kMaxWaves * kMidChunks : kChunks) * kKib || most == kMidChunks * kKib)
+  else if (a.legal || bytes <= (wide || cached ? kMaxWaves * kMidChunks : 32) * kKib)
     p->chunks = kMidChunks;
   else p->chunks = kChunks;
   p->waves = static_cast<int>(up(bytes, p->chunks * kKib));
   // (16-bit rows that start between dwords share their lines' ends with their
   // neighbours: dropped early, those are read twice - 50021 bf16 actions x 2048
   // rows, log probabilities: 42 us kept, 51 us dropped)
-  p->streamed = p->chunks == kChunks && a.n * a.v * size > kLastLevelCache &&
-              (size == 4 || ((reinterpret_cast<uintptr_t>(a.x) | (a.ld * size)) & 3) == 0);
+  p->streamed = p->chunks == kChunks && !cached &&
+                (size == 4 || ((reinterpret_cast<uintptr_t>(a.x) | (a.ld * size)) & 3) == 0);
 }
 
 // Kernels that need the row's sums.
