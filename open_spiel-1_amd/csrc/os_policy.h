@@ -368,6 +368,13 @@ __device__ __forceinline__ float mass_step(const Target& t, float c, float from,
   }
   return from == to ? 1.0f : exp2_((from - to) * c);
 }
+// A mass's share of the total, inv = 1 / total (0: no mass): the quotient with one
+// correction, so that a target with all its mass in one place has q = 1 there and
+// an entropy of 0.
+__device__ __forceinline__ float share(float mass, float total, float inv) {
+  const float q = mass * inv;
+  return fmaf(fmaf(-q, total, mass), inv, q);
+}
 // ln q of a mass share.
 __device__ __forceinline__ float log_share(float q) {
   return kLn2 * fmaxf(__builtin_amdgcn_logf(q), kFloor);
@@ -669,13 +676,15 @@ __device__ __forceinline__ void table_add(const Table& t, int32_t id, float w, f
 
 // p_i (f0 + f1 log2 p_i) of a logit x, as e (g0 + g1 d) with d = x c - R in one
 // operation, e = 2^d and R = m c rounded: what the rounding leaves out and l are
-// in g0 and g1.  A wild row takes d = (x - m) c.
+// in g0 and g1.  A wild row takes d = (x - m) c, and so does every row with kFar
+// (a row's only action then has p = 1 and a gradient of 0).
+template <bool kFar>
 struct Dense {
   float c, ref, m, g0, g1;
   bool plain;  // neither wild nor with a factor that is not finite
   __device__ __forceinline__ Dense(float m_, float l, float c_, float f0, float f1)
       : c(c_), ref(m_ * c_), m(m_) {
-    const bool wild = !(fabsf(ref) <= kWild);
+    const bool wild = kFar || !(fabsf(ref) <= kWild);
     const float k = (wild ? 0.0f : fmaf(-m, c, ref)) - l;
     const float f = exp2_(k);
     g0 = fmaf(f1, k, f0) * f;
@@ -697,7 +706,7 @@ struct Dense {
   template <bool kLog>
   __device__ __forceinline__ float any(float x) const {
     if (x == neg_inf()) return 0.0f;
-    return scaled<kLog>(fabsf(ref) <= kWild ? fmaf(x, c, -ref) : (x - m) * c);
+    return scaled<kLog>(!kFar && fabsf(ref) <= kWild ? fmaf(x, c, -ref) : (x - m) * c);
   }
 };
 
@@ -1143,7 +1152,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
       inv = mass.s == 0.0f ? 0.0f : 1.0f / mass.s;
       if constexpr (kGrad) {
         scale = val.weight * a.inv_t;
-        f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
+        f0 = bad != 0.0f ? __builtin_nanf("") : scale * share(mass.s, mass.s, inv);
       }
     }
     // The entries' part in the loss, and their weights into the table (before the
@@ -1151,7 +1160,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
     [[maybe_unused]] const auto use_targets = [&](const auto& g) {
       float ce = 0.0f, h = 0.0f;
       const auto use = [&](int id, float z, float x) {
-        const float q = target_mass(g.t, a.c, z, mass.z) * inv;
+        const float q = share(target_mass(g.t, a.c, z, mass.z), mass.s, inv);
         if constexpr (kOp != kDistillGrad) {
           if (q != 0.0f) {
             if (id >= 0) ce -= q * log_p(a, x, m, l);
@@ -1240,7 +1249,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
 
     // -- the gradient --
     if constexpr (kGrad) {
-      const Dense dn{m, l, a.c, f0, f1};
+      const Dense<false> dn{m, l, a.c, f0, f1};
       constexpr bool kLog = kOp == kLogprobsGrad;
       T* const gb = static_cast<T*>(g.grad) + r * g.grad_ld + lo;
       const int ln = renewed_scalar(len);
@@ -1289,7 +1298,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
             const bool in = e.id >= lo && e.id < lo + len;
             lid[j] = in ? static_cast<int32_t>(e.id) : -1;
             lx[j] = in ? logit<T>(a, r, e.id) : neg_inf();
-            lw[j] = -scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
+            lw[j] = -scale * share(target_mass(g.t, a.c, e.z, mass.z), mass.s, inv);
           }
           __syncthreads();
           if (tid == 0)
@@ -1615,13 +1624,13 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
       float scale = 0.0f, ce = 0.0f, h = 0.0f;
       if constexpr (kGrad) {
         scale = val.weight * a.inv_t;
-        f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
+        f0 = bad != 0.0f ? __builtin_nanf("") : scale * share(mass.s, mass.s, inv);
       }
       float ew[kGrad ? kHeld : 1];  // the weights, until the values are read
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) {
         if (i * 64 < k) {
-          const float q = target_mass(g.t, a.c, ez[i], mass.z) * inv;
+          const float q = share(target_mass(g.t, a.c, ez[i], mass.z), mass.s, inv);
           const float xi = eid[i] >= 0 ? row[slot(eid[i])] : neg_inf();
           if constexpr (kOp != kDistillGrad) {
             if (q != 0.0f) {
@@ -1638,7 +1647,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
       for (int j = lane + kHeld * 64; j < k; j += 64) {
         const Entry e = target_entry(g.t, r, j);
         const int id = entry_id(e);
-        const float q = target_mass(g.t, a.c, e.z, mass.z) * inv;
+        const float q = share(target_mass(g.t, a.c, e.z, mass.z), mass.s, inv);
         if constexpr (kOp != kDistillGrad) {
           if (q != 0.0f) {
             if (id >= 0) ce -= q * log_p(a, row[slot(id)], m, l);
@@ -1670,7 +1679,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
             const Entry e = target_entry(g.t, r, j);
             const int id = entry_id(e);
             if (id >= 0 && logit<T>(a, r, id) > neg_inf())
-              row[slot(id)] = -scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
+              row[slot(id)] = -scale * share(target_mass(g.t, a.c, e.z, mass.z), mass.s, inv);
           }
         } else {  // in list order
 #pragma unroll
@@ -1685,7 +1694,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
             const Entry e = target_entry(g.t, r, j);
             const int id = entry_id(e);
             if (id >= 0 && logit<T>(a, r, id) > neg_inf())
-              row[slot(id)] -= scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
+              row[slot(id)] -= scale * share(target_mass(g.t, a.c, e.z, mass.z), mass.s, inv);
           }
         }
         fence();
@@ -1730,7 +1739,7 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
     // -- the gradient --
     if constexpr (kGrad) {
       constexpr bool kLog = kOp == kLogprobsGrad;
-      const Dense dn{m, l, a.c, f0, f1};
+      const Dense<false> dn{m, l, a.c, f0, f1};
       T* const gb = static_cast<T*>(g.grad) + r * g.grad_ld;
       renew(me);
 #pragma unroll
@@ -1856,7 +1865,7 @@ __global__ __launch_bounds__(kJoin) void k_join(Rows a, JoinArgs g) {
     float ce = 0.0f, h = 0.0f;
     for (int j = tid; j < q.t.k; j += kJoin) {
       const Entry e = target_entry(q.t, r, j);
-      const float p = target_mass(q.t, a.c, e.z, mass.z) * inv;
+      const float p = share(target_mass(q.t, a.c, e.z, mass.z), mass.s, inv);
       if (p == 0.0f) continue;
       if (e.id >= 0 && e.id < a.v) ce -= p * log_p(a, logit<T>(a, r, e.id), m, l);
       h -= p * log_share(p);
@@ -2009,7 +2018,7 @@ __global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
       float ce = 0.0f, h = 0.0f;
       for (int j = l16; j < g.t.k; j += 16) {
         const Entry e = target_entry(g.t, r, j);
-        const float q = target_mass(g.t, a.c, e.z, mass.z) * inv;
+        const float q = share(target_mass(g.t, a.c, e.z, mass.z), mass.s, inv);
         const bool in = e.id >= 0 && e.id < a.v;
         if constexpr (kOp != kDistillGrad) {
           if (q != 0.0f) {
@@ -2036,9 +2045,9 @@ __global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
           for (int j = 0; j < g.t.k; ++j) {
             const Entry e = target_entry(g.t, r, j);
             if (e.id >= 0 && e.id < a.v)
-              dq[e.id] -= scale * (target_mass(g.t, a.c, e.z, mass.z) * inv);
+              dq[e.id] -= scale * share(target_mass(g.t, a.c, e.z, mass.z), mass.s, inv);
           }
-        f0 = bad != 0.0f ? __builtin_nanf("") : scale * (mass.s * inv);
+        f0 = bad != 0.0f ? __builtin_nanf("") : scale * share(mass.s, mass.s, inv);
         __syncthreads();
       }
     }
@@ -2064,7 +2073,7 @@ __global__ __launch_bounds__(kTinyBlock) void k_tiny(Rows a, ArgsOf<kOp> g) {
       __syncthreads();
     }
     if constexpr (kGrad) {
-      const Dense dn{m, l, a.c, f0, f1};
+      const Dense<true> dn{m, l, a.c, f0, f1};
       T* const gb = static_cast<T*>(g.grad) + r * g.grad_ld;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {

@@ -319,6 +319,53 @@ def test_gpu_distill_odd_targets(require_gpu, v):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("n,v", [(1, 2), (40, 7), (40, 82), (9, 362), (5, 1500), (1100, 5000),
+                                 (2, 150001)])
+def test_gpu_all_mass_in_one_place(require_gpu, n, v, dtype):
+  """A target with one entry, or one that is not 0, has q = 1 there: its entropy
+  is exactly 0."""
+  from os_amd import policy
+  logits, _, _ = make(n, v, dtype, False, seed=11)
+  x = logits.cuda()
+  g = torch.Generator().manual_seed(n + v)
+  ids = torch.randint(0, v, (n, 1), generator=g).cuda()
+  one = (torch.rand(n, 1, generator=g) * 400 + 1e-3).cuda()
+  many = torch.zeros(n, 5, device="cuda")
+  many[:, 2:3] = one
+  for kind, target, at in (("weights", one, ids), ("weights", one.ceil().int(), ids),
+                           ("weights", many, ids.repeat(1, 5)), ("logits", one, ids),
+                           ("logits", many.masked_fill(many == 0, -math.inf), ids.repeat(1, 5))):
+    loss, h = torch.empty(n, device="cuda"), torch.full((n,), -7.0, device="cuda")
+    policy.distill_into(x, target, loss, h, at, kind=kind)
+    assert bool((h == 0).all()), kind
+    grad = torch.empty_like(x)
+    policy.distill_into(x, target, loss, h.fill_(-7), at, kind=kind, grad=grad)
+    assert bool((h == 0).all()), kind
+
+
+@gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("v", [1, 2, 9, 64])
+def test_gpu_forced_moves(require_gpu, v, dtype):
+  """A row's only allowed action has log probability 0, entropy 0, gradient 0."""
+  from os_amd import policy
+  n = 33
+  logits, _, _ = make(n, v, dtype, False, seed=12)
+  moves = torch.arange(n) % v
+  legal = torch.zeros(n, v, dtype=torch.uint8)
+  legal[torch.arange(n), moves] = 1
+  leaf = logits.cuda().requires_grad_()
+  r = policy.logprobs(leaf, moves.cuda(), legal.cuda(), top=1, temperature=0.7)
+  loss, _ = policy.distill(leaf, torch.full((n, 1), 3.0, device="cuda"), moves[:, None].cuda(),
+                           legal.cuda(), temperature=0.7)
+  for x in (r.logprob, r.entropy, r.top_logprob, loss):
+    assert bool((x == 0).all())
+  grad, = torch.autograd.grad((r.logprob * 0.3 + r.entropy - 2 * loss).sum(), leaf)
+  assert bool((grad == 0).all())
+
+
+@gpu
 def test_gpu_strides_and_broadcasts(require_gpu):
   """Row strides of 0 (one row for all), legal [A], legal rows inside wider
   ones, target columns of wider buffers, and memory that starts off any
