@@ -239,7 +239,8 @@ def _own_logprobs(s):
     return r.logprob.detach(), r.entropy.detach(), grad
   policy.logprobs_into(s["logits"], s["entropy"], s["logprob"], s["actions"], s["legal"],
                        s["top_action"], s["top_logprob"], temperature=c["temperature"])
-  return s["logprob"], s["entropy"], s["top_action"], s["top_logprob"]
+  top = min(c["top"], c["v"])  # (past a row's actions: -1 and -inf)
+  return s["logprob"], s["entropy"], s["top_action"][:, :top], s["top_logprob"][:, :top]
 
 
 def _own_distill(s):
