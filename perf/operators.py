@@ -239,8 +239,9 @@ def _own_logprobs(s):
     return r.logprob.detach(), r.entropy.detach(), grad
   policy.logprobs_into(s["logits"], s["entropy"], s["logprob"], s["actions"], s["legal"],
                        s["top_action"], s["top_logprob"], temperature=c["temperature"])
-  top = min(c["top"], c["v"])  # (past a row's actions: -1 and -inf)
-  return s["logprob"], s["entropy"], s["top_action"][:, :top], s["top_logprob"][:, :top]
+  if c["top"] > c["v"]:  # past a row's actions: -1 and -inf, which the plain form leaves out
+    return s["logprob"], s["entropy"], s["top_action"][:, :c["v"]], s["top_logprob"][:, :c["v"]]
+  return s["logprob"], s["entropy"], s["top_action"], s["top_logprob"]
 
 
 def _own_distill(s):
