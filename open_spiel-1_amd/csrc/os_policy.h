@@ -18,7 +18,7 @@
 // ONCE, by whole workgroups, and stays in registers (16 chunks of 16 bytes a
 // lane: up to 256 KiB a workgroup, the register file being 512 KiB a compute
 // unit) from the sums to the gradient or the selection of the top actions.
-// 2048 rows of 131072 bf16 actions: top 20 in 125 us (4.3 TB/s read), loss and
+// 2048 rows of 131072 bf16 actions: top 20 in 124 us (4.3 TB/s read), loss and
 // gradient in 242 us (4.4 TB/s read and written; a copy of 2 GiB: 4.9 TB/s).
 // Short rows (k_wave) are bound by the vector units, few rows by latency.
 // The maximum and the sums run together over the chunks as they arrive (a
