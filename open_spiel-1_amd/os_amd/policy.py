@@ -26,7 +26,8 @@ gradient 0.  A NaN or +inf logit on an allowed action makes its own row's
 results NaN.  Arithmetic is float32; gradients are rounded once to the logits'
 type.  Calls run on the current stream of the logits' device.
 
-Gradients of the first order only.  Capture a training step with the `_into`
+Gradients of the first order and in reverse mode only: a forward-mode tangent
+is refused, not dropped.  Capture a training step with the `_into`
 calls, or with torch.autograd.grad: like any autograd operator, a `.backward()`
 captured while an eager graph of the same leaves is alive is not supported by
 torch.
@@ -36,6 +37,7 @@ from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, lib
@@ -383,7 +385,14 @@ class _Distill(torch.autograd.Function):
     return grad, None, None, None, None, None
 
 
+def _no_tangent(x):
+  # (in any gradient mode: torch.no_grad() leaves forward mode on)
+  if forward_ad.unpack_dual(x).tangent is not None:
+    raise ValueError("forward-mode derivatives are not supported")
+
+
 def _differentiated(logits):
+  _no_tangent(logits)
   return logits.requires_grad and torch.is_grad_enabled()
 
 
@@ -422,6 +431,7 @@ def distill(logits, target, target_actions=None, legal=None, kind="weights", tem
   The loss is 0 for a row without a target, +inf where an excluded action has
   mass, NaN where an action >= A is listed.  The gradient reaches the logits,
   not the target; an excluded action's is 0."""
+  _no_tangent(target)
   if _differentiated(logits):
     return _Distill.apply(logits, target, target_actions, legal, kind, temperature)
   return _new_distill(logits, target, target_actions, legal, kind, temperature, False)[:2]
