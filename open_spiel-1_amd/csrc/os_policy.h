@@ -375,6 +375,15 @@ __device__ __forceinline__ float share(float mass, float total, float inv) {
   const float q = mass * inv;
   return fmaf(fmaf(-q, total, mass), inv, q);
 }
+// Sums taken with d = x c - R, R = m c rounded, hold e0 = 2^off, off = m c - R,
+// where those relative to m hold 1: s becomes share(s, e0, ..), never below 1, and
+// t = sum e d becomes e0 times sum e (x - m) c: the maximum's own e0 off goes as it
+// came, off times the others' sum with it.  So a row's only action has s = 1, t = 0
+// and a log probability and entropy of exactly 0, and no log probability is above 0
+// (2^-off as a factor instead: up to 6e-8 off either way).
+__device__ __forceinline__ float mean_part(float s, float t, float e0, float off) {
+  return fmaf(-off, s - e0, t - e0 * off);
+}
 // ln q of a mass share.
 __device__ __forceinline__ float log_share(float q) {
   return kLn2 * fmaxf(__builtin_amdgcn_logf(q), kFloor);
@@ -676,21 +685,23 @@ __device__ __forceinline__ void table_add(const Table& t, int32_t id, float w, f
 
 // p_i (f0 + f1 log2 p_i) of a logit x, as e (g0 + g1 d) with d = x c - R in one
 // operation, e = 2^d and R = m c rounded: what the rounding leaves out and l are
-// in g0 and g1.  A wild row takes d = (x - m) c, and so does every row with kFar
-// (a row's only action then has p = 1 and a gradient of 0).
+// in g0 and g1.  A wild row takes d = (x - m) c, and so does one whose l is 0 (its
+// only action, or one that leaves the others nothing, then has p = 1 and a
+// gradient of exactly 0) and every row with kFar.
 template <bool kFar>
 struct Dense {
   float c, ref, m, g0, g1;
-  bool plain;  // neither wild nor with a factor that is not finite
+  bool far;    // d = (x - m) c
+  bool plain;  // neither far nor with a factor that is not finite
   __device__ __forceinline__ Dense(float m_, float l, float c_, float f0, float f1)
       : c(c_), ref(m_ * c_), m(m_) {
-    const bool wild = kFar || !(fabsf(ref) <= kWild);
-    const float k = (wild ? 0.0f : fmaf(-m, c, ref)) - l;
+    far = kFar || l == 0.0f || !(fabsf(ref) <= kWild);
+    const float k = (far ? 0.0f : fmaf(-m, c, ref)) - l;
     const float f = exp2_(k);
     g0 = fmaf(f1, k, f0) * f;
     g1 = f1 * f;
     const float inf = __builtin_huge_valf();
-    plain = !wild && fabsf(g0) < inf && fabsf(g1) < inf;
+    plain = !far && fabsf(g0) < inf && fabsf(g1) < inf;
   }
   template <bool kLog>
   __device__ __forceinline__ float scaled(float d) const {
@@ -706,7 +717,7 @@ struct Dense {
   template <bool kLog>
   __device__ __forceinline__ float any(float x) const {
     if (x == neg_inf()) return 0.0f;
-    return scaled<kLog>(!kFar && fabsf(ref) <= kWild ? fmaf(x, c, -ref) : (x - m) * c);
+    return scaled<kLog>(kFar || far ? (x - m) * c : fmaf(x, c, -ref));
   }
 };
 
@@ -938,13 +949,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
       }
     }
 
-    // from R to the lane's exact m c
+    // from R to the lane's exact m c (see mean_part())
     if constexpr (kSums) {
       if (ref > -kWild) {
-        const float off = fmaf(u.m, a.c, -ref);
-        const float f = exp2_(-off);
-        if constexpr (kEnt) u.t = f * fmaf(-off, u.s, u.t);
-        u.s *= f;
+        const float off = fmaf(u.m, a.c, -ref), e0 = exp2_(off), inv = __builtin_amdgcn_rcpf(e0);
+        if constexpr (kEnt) u.t = inv * mean_part(u.s, u.t, e0, off);
+        u.s = share(u.s, e0, inv);
       }
     }
 
@@ -1461,10 +1471,11 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
       for (int i = 0; i < kX; ++i) lane_max = fmaxf(lane_max, x[i]);
       m = fold64(lane_max, Max{});
       if (m == neg_inf()) m = 0.0f;  // empty, or only NaN
-      float s = 0.0f, u = 0.0f, off = 0.0f;
+      float s = 0.0f, u = 0.0f, off = 0.0f, e0 = 1.0f;
       const float ref = m * a.c;
       if (fabsf(ref) <= kWild) {
         off = fmaf(m, a.c, -ref);
+        e0 = exp2_(off);
 #pragma unroll
         for (int i = 0; i < kX; ++i) {
           const float d = fmaf(x[i], a.c, -ref);
@@ -1482,8 +1493,8 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
         }
       }
       s = fold64(s, Add{});
-      l = s == 0.0f ? 0.0f : log2f(s) - off;
-      if constexpr (kLp) mean = s == 0.0f ? 0.0f : fold64(u, Add{}) / s - off;
+      l = s == 0.0f ? 0.0f : log2f(share(s, e0, __builtin_amdgcn_rcpf(e0)));
+      if constexpr (kLp) mean = s == 0.0f ? 0.0f : mean_part(s, fold64(u, Add{}), e0, off) / s;
     } else {
       m = val.m;
       l = val.l;

@@ -49,3 +49,53 @@ def test_gpu_forward_mode_is_refused(require_gpu):
     policy.distill(x, t)
   with pytest.raises(ValueError, match="forward-mode"):
     torch.func.jvp(lambda z: policy.distill(z, t)[0], (x,), (t,))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("v", [65, 82, 130, 362, 500, 768, 1025, 1400, 2047, 2049, 4099, 20011, 33001,
+                               70001, 150001, 300007])
+def test_gpu_forced_moves_of_long_rows(require_gpu, v, dtype):
+  """A row's only allowed action has log probability 0, entropy 0, gradient 0,
+  whichever kernel takes it, whether a mask or logits of -inf exclude the rest;
+  few rows and many go through different ones."""
+  from os_amd import policy
+  n = 33 if v < 33000 else 3
+  logits, _, _ = make(n, v, dtype, False, seed=21, spread=1.0)
+  logits[1:] *= 9
+  moves = (torch.arange(n) * 7919 + v - 1) % v
+  legal = torch.zeros(n, v, dtype=torch.uint8)
+  legal[torch.arange(n), moves] = 1
+  alone = logits.masked_fill(legal == 0, -math.inf)
+  ids, one = moves[:, None].cuda(), torch.full((n, 1), 3.0, device="cuda")
+  for x, lg in ((logits, legal.cuda()), (alone, None)):
+    for t in (1.0, 0.7):
+      leaf = x.cuda().requires_grad_()
+      r = policy.logprobs(leaf, moves.cuda(), lg, top=1, temperature=t)
+      loss, _ = policy.distill(leaf, one, ids, lg, temperature=t)
+      for what, got in (("logprob", r.logprob), ("entropy", r.entropy), ("top", r.top_logprob),
+                        ("loss", loss)):
+        assert bool((got == 0).all()), (what, t, got[got != 0][:4])
+      grad, = torch.autograd.grad((r.logprob * 0.3 + r.entropy - 2 * loss).sum(), leaf)
+      assert bool((grad == 0).all())
+      both, loss = torch.empty_like(leaf), torch.empty(n, device="cuda")
+      policy.distill_into(leaf.detach(), one, loss, None, ids, lg, temperature=t, grad=both)
+      assert bool((loss == 0).all()) and bool((both == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("v", [64, 65, 362, 700, 1500, 2049, 5000, 150001])
+def test_gpu_log_probabilities_are_not_positive(require_gpu, v):
+  """Rows whose likeliest action is far ahead: its probability is 1 within a few
+  steps, its log probability never above 0."""
+  from os_amd import policy
+  n = 400 if v < 100000 else 40
+  g = torch.Generator(device="cuda").manual_seed(v)
+  x = torch.randn(n, v, generator=g, device="cuda") + torch.randn(n, 1, generator=g, device="cuda") * 5
+  best = torch.randint(0, v, (n,), generator=g, device="cuda")
+  x[torch.arange(n, device="cuda"), best] += 30.0
+  for t in (1.0, 0.7):
+    r = policy.logprobs(x, best, top=2, temperature=t)
+    assert bool((r.logprob <= 0).all()) and bool((r.top_logprob <= 0).all())
+    loss, _ = policy.distill(x, torch.ones(n, 1, device="cuda"), best[:, None], temperature=t)
+    assert bool((loss >= 0).all())
