@@ -443,9 +443,11 @@ int os_az_logprobs_grad_async(const os_az_rows* rows, const void* actions, int32
                                   int64_t grad_ld, void* hip_stream);
 /* loss[r] = -sum_j q_j log p[a_j], the cross entropy (+inf when an excluded
  * action has mass, NaN when a listed action is >= num_actions; 0 when the row
- * has no target), target_entropy[r] = -sum_j q_j log q_j (loss - target_entropy
- * is the Kullback-Leibler divergence; NULL: not wanted), stats as above (NULL:
- * not wanted).  grad != NULL: grad[r][i] = weight[r] d loss[r] / d logits[r][i]
+ * has no target), target_entropy[r] = -sum_j q_j log q_j over the entries as
+ * listed (NULL: not wanted; where a row's actions are distinct, loss -
+ * target_entropy is the Kullback-Leibler divergence from the target; an action
+ * listed more than once adds the entropy of its split into entries), stats as
+ * above (NULL: not wanted).  grad != NULL: grad[r][i] = weight[r] d loss[r] / d logits[r][i]
  * = weight[r] (p_i sum q - q_i) / temperature, 0 where the action is excluded;
  * weight NULL: 1. */
 int os_az_distill_async(const os_az_rows* rows, const os_az_target* target,

@@ -418,8 +418,11 @@ def logprobs(logits, actions=None, legal=None, top=0, temperature=1.0):
 def distill(logits, target, target_actions=None, legal=None, kind="weights", temperature=1.0):
   """(loss, target_entropy), float32 [N]: the cross entropy -sum_j q_j log p of
   the policies softmax(logits / temperature) over the allowed actions against
-  the target distribution q, and q's entropy; loss - target_entropy is the
-  Kullback-Leibler divergence from q.
+  the target distribution q, and the entropy -sum_j q_j log q_j of q's entries as
+  they are listed.  Where a row's actions are distinct, loss - target_entropy is
+  the Kullback-Leibler divergence from q; an action listed more than once adds
+  the entropy of its split, so merge repeats first for a divergence (the loss and
+  its gradient are the same either way).
 
   Entry j of row r is action target_actions[r, j] (int32 or int64 [N, K], K <=
   1024; negative: padding; listed twice counts twice) with target[r, j], which

@@ -99,3 +99,60 @@ def test_gpu_log_probabilities_are_not_positive(require_gpu, v):
     assert bool((r.logprob <= 0).all()) and bool((r.top_logprob <= 0).all())
     loss, _ = policy.distill(x, torch.ones(n, 1, device="cuda"), best[:, None], temperature=t)
     assert bool((loss >= 0).all())
+
+
+def _merged(ids, q, v):
+  """The target distribution over the actions (64 bits): repeats added up."""
+  full = torch.zeros(len(q), v, dtype=torch.float64)
+  return full.scatter_add_(1, ids.clamp(min=0).long(), torch.where(ids >= 0, q, torch.zeros_like(q)))
+
+
+@gpu
+@pytest.mark.parametrize("repeats", [False, True])
+@pytest.mark.parametrize("v", [40, 700, 3000, 150001])
+def test_gpu_target_entropy_is_that_of_the_entries(require_gpu, v, repeats):
+  """target_entropy = -sum_j q_j log q_j over the listed entries.  With distinct
+  actions loss - target_entropy is the divergence of the target distribution from
+  the policy; an action listed m times with mass Q in all leaves it short of that
+  by sum Q log m or less, which the entries' entropy has too much."""
+  from os_amd import policy
+  n, k = 6, 12
+  logits, _, _ = make(n, v, "f32", False, seed=31)
+  g = torch.Generator().manual_seed(v)
+  ids = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(n)])
+  if repeats:
+    ids = ids[:, torch.arange(k) // 3]
+  w = torch.rand(n, k, generator=g) + 0.1
+  loss, h = policy.distill(logits.cuda(), w.cuda(), ids.cuda())
+  want, tol = ref.distill(logits, w, ids)
+  close(loss, want["loss"], tol["loss"], "loss")
+  close(h, want["entropy"], tol["entropy"], "entropy")
+  q = w.double() / w.double().sum(1, keepdim=True)
+  full = _merged(ids, q, v)
+  merged = -torch.special.xlogy(full, full).sum(1)
+  _, logp = ref.softmax(logits.double())
+  divergence = torch.special.xlogy(full, full).sum(1) - (full * logp).sum(1)
+  assert bool((divergence > 0).all())
+  got = (loss - h).cpu().double()
+  # (the subtraction's own rounding: half a step of the result)
+  bound = tol["loss"] + tol["entropy"] + got.abs() * ref.U
+  if repeats:
+    assert bool((h.cpu().double() > merged + bound).all()) and bool((got < divergence - bound).all())
+    assert bool((got > divergence - math.log(3) - bound).all())
+  else:
+    assert bool(((got - divergence).abs() <= bound).all())
+
+
+def test_the_divergence_is_stated_for_distinct_actions():
+  """(two equal logits, the first action listed four times: loss log 2, entropy of
+  the entries log 4)"""
+  import os
+  import re
+  from os_amd import policy
+  root = os.path.join(os.path.dirname(__file__), "..")
+  texts = [policy.distill.__doc__, open(os.path.join(root, "include", "os_mcts.h")).read(),
+           open(os.path.join(root, "INTEGRATION.md")).read()]
+  for text in texts:
+    text = re.sub(r"[\s*]+", " ", text)
+    at = text.index("Kullback-Leibler")
+    assert "distinct" in text[max(0, at - 200):at + 200]
