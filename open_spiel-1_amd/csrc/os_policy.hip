@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 #include "os_error.h"
@@ -190,6 +191,69 @@ int check_workspace(int64_t need, const void* workspace, int64_t bytes) {
   return OS_OK;
 }
 
+// A call's buffer: `n` rows of `bytes` bytes, `ld` bytes apart.
+struct Buffer {
+  const char* name;
+  const void* p;
+  int64_t n, ld, bytes;
+  bool out;
+};
+
+// [first, past) of the buffer (a stride so large that it leaves 64 bits: to the end).
+uint64_t past(const Buffer& b) {
+  uint64_t far, end;
+  const uint64_t at = reinterpret_cast<uintptr_t>(b.p);
+  if (__builtin_mul_overflow(static_cast<uint64_t>(b.n - 1), static_cast<uint64_t>(b.ld), &far) ||
+      __builtin_add_overflow(far, at + static_cast<uint64_t>(b.bytes), &end))
+    return UINT64_MAX;
+  return end;
+}
+
+bool overlap(const Buffer& a, const Buffer& b) {
+  const uint64_t a0 = reinterpret_cast<uintptr_t>(a.p), b0 = reinterpret_cast<uintptr_t>(b.p);
+  if (a0 >= past(b) || b0 >= past(a)) return false;
+  if (a.ld != b.ld || a.ld == 0) return true;
+  // fine as disjoint columns of one buffer's rows
+  const uint64_t ld = static_cast<uint64_t>(a.ld);
+  const uint64_t off = b0 >= a0 ? (b0 - a0) % ld : (ld - (a0 - b0) % ld) % ld;
+  return off < static_cast<uint64_t>(a.bytes) || off + static_cast<uint64_t>(b.bytes) > ld;
+}
+
+// Results share no memory with each other or with what the call reads: rows are
+// worked on in any order, and some operands are read again after a result is
+// written.
+int check_apart(std::initializer_list<Buffer> all) {
+  const auto there = [](const Buffer& b) { return b.p != nullptr && b.n > 0 && b.bytes > 0; };
+  for (const Buffer* a = all.begin(); a != all.end(); ++a) {
+    if (!a->out || !there(*a)) continue;
+    for (const Buffer* b = all.begin(); b != all.end(); ++b)
+      if (a != b && (!b->out || a < b) && there(*b) && overlap(*a, *b))
+        return Fail(OS_ERR_INVALID, std::string(a->name) + " overlaps " + b->name);
+  }
+  return OS_OK;
+}
+
+// `bytes` a row, rows end to end.
+Buffer per_row(const char* name, const void* p, const Rows& a, int64_t bytes, bool out = false) {
+  return Buffer{name, p, 1, 0, a.n * bytes, out};
+}
+Buffer strided(const char* name, const void* p, const Rows& a, int64_t stride) {
+  return Buffer{name, p, a.n, stride * 4, 4, false};
+}
+Buffer matrix(const char* name, const void* p, const Rows& a, int64_t ld, int64_t columns, int64_t size,
+              bool out = false) {
+  return Buffer{name, p, a.n, ld * size, columns * size, out};
+}
+Buffer logits_of(const Rows& a, int size) { return matrix("logits", a.x, a, a.ld, a.v, size); }
+Buffer legal_of(const Rows& a) { return matrix("legal", a.legal, a, a.lld, a.v, 1); }
+Buffer ids_of(const Rows& a, const Target& t) {
+  return matrix("target actions", t.ids, a, t.ids_ld, t.k, t.wide ? 8 : 4);
+}
+Buffer values_of(const Rows& a, const Target& t) {
+  const bool half = t.type == OS_AZ_LOGITS_BF16 || t.type == OS_AZ_LOGITS_F16;
+  return matrix("target", t.val, a, t.val_ld, t.k, half ? 2 : 4);
+}
+
 // Fail() keeps its message in a string, which may run out of memory: nothing
 // leaves a C entry but a code.
 template <class F>
@@ -232,6 +296,14 @@ int os_az_logprobs_async(const os_az_rows* rows, const void* actions, int32_t wi
     const Plan p = sums_plan(a, type_size(rows->dtype));
     const int64_t need = workspace_bytes_of(a, p, top);
     if (const int rc = check_workspace(need, workspace, workspace_bytes)) return rc;
+    if (const int rc = check_apart(
+            {logits_of(a, type_size(rows->dtype)), legal_of(a), per_row("actions", actions, a, wide ? 8 : 4),
+             per_row("logprob", logprob, a, 4, true), per_row("entropy", entropy, a, 4, true),
+             per_row("stats", stats, a, 8, true),
+             per_row("top_action", top_action, a, int64_t{8} * top, true),
+             per_row("top_logprob", top_logprob, a, int64_t{4} * top, true),
+             Buffer{"workspace", workspace, 1, 0, need, true}}))
+      return rc;
     LogprobArgs g{actions, wide != 0, top, logprob, entropy, stats, top_action, top_logprob,
                   nullptr, nullptr};
     if (need > 0) {
@@ -264,7 +336,16 @@ int os_az_logprobs_grad_async(const os_az_rows* rows, const void* actions, int32
       return Fail(OS_ERR_INVALID, "null gradient buffer");
     if (!g_top) top = 0;
     if (top > 0 && !top_action) return Fail(OS_ERR_INVALID, "null top_action");
-    const Plan p = grad_plan(a, type_size(rows->dtype));
+    const int size = type_size(rows->dtype);
+    if (const int rc = check_apart(
+            {logits_of(a, size), legal_of(a), per_row("actions", actions, a, wide ? 8 : 4),
+             per_row("entropy", g_entropy ? entropy : nullptr, a, 4), per_row("stats", stats, a, 8),
+             per_row("top_action", top_action, a, int64_t{8} * top),
+             strided("g_logprob", g_logprob, a, g_logprob_stride),
+             strided("g_entropy", g_entropy, a, g_entropy_stride),
+             per_row("g_top", g_top, a, int64_t{4} * top), matrix("grad", grad, a, grad_ld, a.v, size, true)}))
+      return rc;
+    const Plan p = grad_plan(a, size);
     const LogprobGradArgs g{actions,    wide != 0,        top,       entropy,          stats,
                             top_action, g_logprob,        g_logprob_stride, g_entropy, g_entropy_stride,
                             g_top,      grad,             grad_ld};
@@ -294,6 +375,13 @@ int os_az_distill_async(const os_az_rows* rows, const os_az_target* target, cons
     const int64_t need = workspace_bytes_of(a, p, 0);
     const bool parts = need > 0;
     if (const int rc = check_workspace(need, workspace, workspace_bytes)) return rc;
+    if (const int rc = check_apart(
+            {logits_of(a, size), legal_of(a), ids_of(a, t), values_of(a, t),
+             per_row("weight", grad ? weight : nullptr, a, 4), per_row("loss", loss, a, 4, true),
+             per_row("target_entropy", target_entropy, a, 4, true), per_row("stats", stats, a, 8, true),
+             matrix("grad", grad, a, grad_ld, a.v, size, true),
+             Buffer{"workspace", workspace, 1, 0, need, true}}))
+      return rc;
     DistillArgs g{t, weight, 1, loss, target_entropy, stats, grad, grad_ld, 0};
     return by_dtype(rows->dtype, [&](auto k) {
       Launch c = launch(a, p, hip_stream);
@@ -329,7 +417,13 @@ int os_az_distill_grad_async(const os_az_rows* rows, const os_az_target* target,
     if (const int rc = check_grad(a, rows->dtype, grad, grad_ld)) return rc;
     if (a.n == 0) return OS_OK;
     if (!stats || !grad) return Fail(OS_ERR_INVALID, "null gradient buffer");
-    const Plan p = grad_plan(a, type_size(rows->dtype));
+    const int size = type_size(rows->dtype);
+    if (const int rc = check_apart({logits_of(a, size), legal_of(a), ids_of(a, t), values_of(a, t),
+                                    strided("weight", weight, a, weight_stride),
+                                    per_row("stats", stats, a, 8),
+                                    matrix("grad", grad, a, grad_ld, a.v, size, true)}))
+      return rc;
+    const Plan p = grad_plan(a, size);
     DistillArgs g{t, weight, weight_stride, nullptr, nullptr, const_cast<float*>(stats),
                   grad, grad_ld, 0};
     return by_dtype(rows->dtype, [&](auto k) {

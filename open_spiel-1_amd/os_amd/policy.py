@@ -182,25 +182,19 @@ def _grad_buffer(grad, logits, n, a, dev):
   ld, step = grad.stride()
   if (step != 1 and a > 1) or (ld < a and n > 1):
     raise ValueError("grad must have unit column stride and rows that do not overlap")
-  ld = max(ld, a)
-  g0 = grad.data_ptr()
-  if n > 0:
-    size, x0, x_ld = grad.element_size(), logits.data_ptr(), logits.stride(0)
-    if (g0 < x0 + ((n - 1) * x_ld + a) * size and x0 < g0 + ((n - 1) * ld + a) * size):
-      # their extents meet: fine as disjoint columns of one buffer's rows
-      off = (g0 - x0) // size % ld
-      if x_ld != ld or off < a or off + a > ld:
-        raise ValueError("grad overlaps the logits")
-  return g0, ld
+  return grad.data_ptr(), max(ld, a)
 
 
 def _launch(fn, dev, *args):
-  """Calls a C entry on the device's current stream."""
+  """Calls a C entry on the device's current stream (it also refuses results that
+  overlap each other or an operand)."""
   if dev == torch.cuda.current_device():
     rc = fn(*args, _raw_stream(dev))
   else:
     with torch.cuda.device(dev):
       rc = fn(*args, _raw_stream(dev))
+  if rc == _lib.OS_ERR_INVALID:
+    raise ValueError(lib.os_last_error().decode(errors="replace"))
   if rc:
     check(rc)
 

@@ -156,3 +156,102 @@ def test_the_divergence_is_stated_for_distinct_actions():
     text = re.sub(r"[\s*]+", " ", text)
     at = text.index("Kullback-Leibler")
     assert "distinct" in text[max(0, at - 200):at + 200]
+
+
+def test_abi_refuses_overlapping_buffers():
+  """A result that shares memory with an operand or another result, before any
+  launch: each pair of a call's buffers in turn, disjoint columns of one buffer's
+  rows let by (those calls fail later, at the launch: there is no GPU here)."""
+  import ctypes
+  from os_amd import _lib
+  L = _lib.lib
+  n, v, k, top = 4, 40000, 3, 2
+  base = 1 << 20
+
+  def at(i):
+    return base * (1 + 2 * i)
+  size = {"logits": n * v * 4, "legal": n * v, "actions": n * 8, "logprob": n * 4, "entropy": n * 4,
+          "stats": n * 8, "top_action": n * top * 8, "top_logprob": n * top * 4, "g_logprob": n * 4,
+          "g_entropy": n * 4, "g_top": n * top * 4, "grad": n * v * 4, "ids": n * k * 8,
+          "target": n * k * 4, "weight": n * 4, "loss": n * 4, "target_entropy": n * 4}
+  assert max(size.values()) <= base
+
+  def call(name, p):
+    rows = ctypes.byref(_lib.AzRows(logits=p["logits"], legal=p["legal"], num_rows=n, ld=v,
+                                    legal_ld=v, num_actions=v, dtype=0, temperature=1.0))
+    tg = None
+    if "ids" in p:
+      tg = ctypes.byref(_lib.AzTarget(actions=p["ids"], target=p["target"], actions_ld=k,
+                                      target_ld=k, k=k, type=3, wide=1))
+    if name == "logprobs":
+      work = L.os_az_rows_workspace(rows, top)
+      return L.os_az_logprobs_async(rows, p["actions"], 1, p["logprob"], p["entropy"], p["stats"], top,
+                                    p["top_action"], p["top_logprob"], at(40), work, None)
+    if name == "logprobs_grad":
+      return L.os_az_logprobs_grad_async(rows, p["actions"], 1, p["entropy"], p["stats"], top,
+                                         p["top_action"], p["g_logprob"], 1, p["g_entropy"], 1,
+                                         p["g_top"], p["grad"], v, None)
+    if name == "distill":
+      work = L.os_az_rows_workspace(rows, 0)
+      return L.os_az_distill_async(rows, tg, p["weight"], p["loss"], p["target_entropy"], p["stats"],
+                                   p["grad"], v, at(40), work, None)
+    return L.os_az_distill_grad_async(rows, tg, p["weight"], 1, p["stats"], p["grad"], v, None)
+  calls = {
+      "logprobs": (["logits", "legal", "actions"],
+                   ["logprob", "entropy", "stats", "top_action", "top_logprob"]),
+      "logprobs_grad": (["logits", "legal", "actions", "entropy", "stats", "top_action", "g_logprob",
+                         "g_entropy", "g_top"], ["grad"]),
+      "distill": (["logits", "legal", "ids", "target", "weight"],
+                  ["loss", "target_entropy", "stats", "grad"]),
+      "distill_grad": (["logits", "legal", "ids", "target", "weight", "stats"], ["grad"]),
+  }
+  for name, (ins, outs) in calls.items():
+    names = ins + outs
+    for o in outs:
+      for other in names:
+        if other == o:
+          continue
+        for shift in (0, size[other] - 8, 8 - size[o]):
+          p = {x: at(i) for i, x in enumerate(names)}
+          p[o] = p[other] + shift
+          assert call(name, p) == _lib.OS_ERR_INVALID, (name, o, other, shift)
+          assert b"overlap" in L.os_last_error(), (name, o, other, shift, L.os_last_error())
+
+
+@gpu
+def test_gpu_overlapping_results_are_refused(require_gpu):
+  """From Python: ValueError; neighbours and disjoint columns are no overlap."""
+  from os_amd import policy
+  n, a = 6, 9
+  f = dict(device="cuda")
+  x, t = torch.zeros(n, a, **f), torch.rand(n, a, **f)
+  legal = torch.ones(n, a, dtype=torch.uint8, **f)
+  out, h = torch.zeros(n, **f), torch.zeros(n, **f)
+  act = torch.zeros(n, dtype=torch.int64, **f)
+  w = torch.ones(n, **f)
+  buf = torch.zeros(3 * n * a, **f)
+  ta = torch.zeros(n, 3, dtype=torch.int64, **f)
+  for call in (lambda: policy.distill_into(x, t, out, None, None, grad=t),
+               lambda: policy.distill_into(x, t, out, out),
+               lambda: policy.distill_into(x, t, w, None, weight=w, grad=torch.empty_like(x)),
+               lambda: policy.distill_into(x, t, t.view(-1)[:n]),
+               lambda: policy.logprobs_into(x, x.view(-1)[:n]),
+               lambda: policy.logprobs_into(x, out, out, act),
+               lambda: policy.logprobs_into(x, out, act.view(torch.float32)[:n], act),
+               lambda: policy.logprobs_into(x, out, top_action=ta,
+                                            top_logprob=ta.view(-1).view(torch.float32)[:18].view(n, 3)),
+               lambda: policy.logprobs_into(x, buf[:n], stats=buf[2:2 * n + 2].view(n, 2))):
+    with pytest.raises(ValueError):
+      call()
+  # one buffer's neighbouring parts
+  policy.logprobs_into(x, buf[:n], buf[n:2 * n], act, stats=buf[2 * n:4 * n].view(n, 2))
+  both = torch.zeros(n, 3 * a, **f)
+  both[:, a:2 * a] = t
+  policy.distill_into(both[:, :a], both[:, a:2 * a], out, h, grad=both[:, 2 * a:])
+  want, tol = ref.distill(x.cpu(), t.cpu())
+  close(out, want["loss"], tol["loss"], "loss")
+  close(both[:, 2 * a:], want["grad"], tol["grad"] + ref.rounding(torch.float32, want["grad"]), "grad")
+  rows = torch.zeros(2 * n, a, **f)
+  policy.distill_into(rows[::2], t, out, h, grad=rows[1::2])
+  close(rows[1::2], want["grad"], tol["grad"] + ref.rounding(torch.float32, want["grad"]), "grad")
+  assert bool((rows[::2] == 0).all())
