@@ -65,6 +65,11 @@ except AttributeError:
   def _raw_stream(device):
     return torch.cuda.current_stream(device).cuda_stream
 
+try:  # its check of the argument takes three times as long as the rest
+  _increment_version = torch._C._increment_version
+except AttributeError:
+  _increment_version = torch.autograd.graph.increment_version
+
 
 class LogProbs(NamedTuple):
   """Results of logprobs (float32; top_action int64)."""
@@ -199,6 +204,12 @@ def _launch(fn, dev, *args):
     check(rc)
 
 
+def _written(*out):
+  """Autograd learns that a call wrote these (those that there are): a graph that
+  saved one of them before refuses to run backward."""
+  _increment_version([x for x in out if x is not None])
+
+
 def _workspace(rows, a, top, dev):
   """(tensor to keep until the call, address, bytes): rows of few actions need
   none (os_az_rows_workspace)."""
@@ -239,6 +250,7 @@ def logprobs_into(logits, entropy, logprob=None, actions=None, legal=None, top_a
   h = _like("entropy", entropy, dev, _F32, n)
   keep, work, size = _workspace(rows, a, top, dev)
   _launch(lib.os_az_logprobs_async, dev, rows, act, wide, lp, h, st, top, ta, tl, work, size)
+  _written(entropy, logprob, stats, top_action, top_logprob)
   del keep
 
 
@@ -261,6 +273,7 @@ def distill_into(logits, target, loss, target_entropy=None, target_actions=None,
   st = None if stats is None else _like("stats", stats, dev, _F32, n, 2)
   keep, work, size = _workspace(rows, a, 0, dev)
   _launch(lib.os_az_distill_async, dev, rows, t, w, out, h, st, g, ld, work, size)
+  _written(loss, target_entropy, stats, grad)
   del keep
 
 

@@ -255,3 +255,42 @@ def test_gpu_overlapping_results_are_refused(require_gpu):
   policy.distill_into(rows[::2], t, out, h, grad=rows[1::2])
   close(rows[1::2], want["grad"], tol["grad"] + ref.rounding(torch.float32, want["grad"]), "grad")
   assert bool((rows[::2] == 0).all())
+
+
+@gpu
+def test_gpu_written_tensors_change_their_version(require_gpu):
+  """Autograd finds out that a tensor which an older graph has saved was written
+  by logprobs_into or distill_into since."""
+  from os_amd import policy
+  n, a = 6, 9
+  f = dict(device="cuda")
+  x, t, w = torch.randn(n, a, **f), torch.rand(n, a, **f), torch.ones(n, **f)
+  act = torch.zeros(n, dtype=torch.int64, **f)
+
+  def new():
+    return dict(entropy=torch.ones(n, **f), logprob=torch.ones(n, **f), stats=torch.ones(n, 2, **f),
+                top_action=torch.zeros(n, 2, dtype=torch.int64, **f), top_logprob=torch.ones(n, 2, **f)), \
+        dict(loss=torch.ones(n, **f), target_entropy=torch.ones(n, **f), grad=torch.ones(n, a, **f),
+             stats=torch.ones(n, 2, **f))
+  lp, ds = new()
+  calls = ((lp, lambda o: policy.logprobs_into(x, actions=act, **o)),
+           (ds, lambda o: policy.distill_into(x, t, weight=w, **o)))
+  for out, call in calls:
+    for key, tensor in out.items():
+      scale = torch.ones_like(tensor, dtype=torch.float32).requires_grad_()
+      before = tensor._version
+      graph = (scale * tensor).sum()
+      call(out)
+      assert tensor._version > before, key
+      if tensor.is_floating_point():
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+          graph.backward()
+  # operands are not written
+  assert x._version == t._version == w._version == act._version == 0
+  # tensors made in inference mode have no version, and are written all the same
+  with torch.inference_mode():
+    lp, ds = new()
+  policy.logprobs_into(x, actions=act, **lp)
+  policy.distill_into(x, t, weight=w, **ds)
+  want, tol = ref.distill(x.cpu(), t.cpu())
+  close(ds["loss"], want["loss"], tol["loss"], "loss")
