@@ -191,11 +191,12 @@ int check_workspace(int64_t need, const void* workspace, int64_t bytes) {
   return OS_OK;
 }
 
-// A call's buffer: `n` rows of `bytes` bytes, `ld` bytes apart.
+// A call's buffer: `n` rows of `bytes` bytes in elements of `size`, `ld` bytes apart.
 struct Buffer {
   const char* name;
   const void* p;
   int64_t n, ld, bytes;
+  int size;
   bool out;
 };
 
@@ -219,13 +220,17 @@ bool overlap(const Buffer& a, const Buffer& b) {
   return off < static_cast<uint64_t>(a.bytes) || off + static_cast<uint64_t>(b.bytes) > ld;
 }
 
-// Results share no memory with each other or with what the call reads: rows are
-// worked on in any order, and some operands are read again after a result is
-// written.
-int check_apart(std::initializer_list<Buffer> all) {
+// Elements lie at multiples of their size (a row's single values are scalar
+// loads, which drop an address's low bits).  Results share no memory with each
+// other or with what the call reads: rows are worked on in any order, and some
+// operands are read again after a result is written.
+int check_buffers(std::initializer_list<Buffer> all) {
   const auto there = [](const Buffer& b) { return b.p != nullptr && b.n > 0 && b.bytes > 0; };
   for (const Buffer* a = all.begin(); a != all.end(); ++a) {
-    if (!a->out || !there(*a)) continue;
+    if (!there(*a)) continue;
+    if (reinterpret_cast<uintptr_t>(a->p) & static_cast<uintptr_t>(a->size - 1))
+      return Fail(OS_ERR_INVALID, std::string(a->name) + " not aligned to its type");
+    if (!a->out) continue;
     for (const Buffer* b = all.begin(); b != all.end(); ++b)
       if (a != b && (!b->out || a < b) && there(*b) && overlap(*a, *b))
         return Fail(OS_ERR_INVALID, std::string(a->name) + " overlaps " + b->name);
@@ -233,16 +238,19 @@ int check_apart(std::initializer_list<Buffer> all) {
   return OS_OK;
 }
 
-// `bytes` a row, rows end to end.
-Buffer per_row(const char* name, const void* p, const Rows& a, int64_t bytes, bool out = false) {
-  return Buffer{name, p, 1, 0, a.n * bytes, out};
+// `each` elements a row, rows end to end.
+Buffer per_row(const char* name, const void* p, const Rows& a, int size, int64_t each) {
+  return Buffer{name, p, 1, 0, a.n * each * size, size, false};
 }
 Buffer strided(const char* name, const void* p, const Rows& a, int64_t stride) {
-  return Buffer{name, p, a.n, stride * 4, 4, false};
+  return Buffer{name, p, a.n, stride * 4, 4, 4, false};
 }
-Buffer matrix(const char* name, const void* p, const Rows& a, int64_t ld, int64_t columns, int64_t size,
-              bool out = false) {
-  return Buffer{name, p, a.n, ld * size, columns * size, out};
+Buffer matrix(const char* name, const void* p, const Rows& a, int64_t ld, int64_t columns, int size) {
+  return Buffer{name, p, a.n, ld * size, columns * size, size, false};
+}
+Buffer result(Buffer b) {
+  b.out = true;
+  return b;
 }
 Buffer logits_of(const Rows& a, int size) { return matrix("logits", a.x, a, a.ld, a.v, size); }
 Buffer legal_of(const Rows& a) { return matrix("legal", a.legal, a, a.lld, a.v, 1); }
@@ -253,6 +261,7 @@ Buffer values_of(const Rows& a, const Target& t) {
   const bool half = t.type == OS_AZ_LOGITS_BF16 || t.type == OS_AZ_LOGITS_F16;
   return matrix("target", t.val, a, t.val_ld, t.k, half ? 2 : 4);
 }
+Buffer workspace_of(const void* p, int64_t bytes) { return Buffer{"workspace", p, 1, 0, bytes, 16, true}; }
 
 // Fail() keeps its message in a string, which may run out of memory: nothing
 // leaves a C entry but a code.
@@ -296,13 +305,11 @@ int os_az_logprobs_async(const os_az_rows* rows, const void* actions, int32_t wi
     const Plan p = sums_plan(a, type_size(rows->dtype));
     const int64_t need = workspace_bytes_of(a, p, top);
     if (const int rc = check_workspace(need, workspace, workspace_bytes)) return rc;
-    if (const int rc = check_apart(
-            {logits_of(a, type_size(rows->dtype)), legal_of(a), per_row("actions", actions, a, wide ? 8 : 4),
-             per_row("logprob", logprob, a, 4, true), per_row("entropy", entropy, a, 4, true),
-             per_row("stats", stats, a, 8, true),
-             per_row("top_action", top_action, a, int64_t{8} * top, true),
-             per_row("top_logprob", top_logprob, a, int64_t{4} * top, true),
-             Buffer{"workspace", workspace, 1, 0, need, true}}))
+    if (const int rc = check_buffers(
+            {logits_of(a, type_size(rows->dtype)), legal_of(a), per_row("actions", actions, a, wide ? 8 : 4, 1),
+             result(per_row("logprob", logprob, a, 4, 1)), result(per_row("entropy", entropy, a, 4, 1)),
+             result(per_row("stats", stats, a, 4, 2)), result(per_row("top_action", top_action, a, 8, top)),
+             result(per_row("top_logprob", top_logprob, a, 4, top)), workspace_of(workspace, need)}))
       return rc;
     LogprobArgs g{actions, wide != 0, top, logprob, entropy, stats, top_action, top_logprob,
                   nullptr, nullptr};
@@ -337,13 +344,12 @@ int os_az_logprobs_grad_async(const os_az_rows* rows, const void* actions, int32
     if (!g_top) top = 0;
     if (top > 0 && !top_action) return Fail(OS_ERR_INVALID, "null top_action");
     const int size = type_size(rows->dtype);
-    if (const int rc = check_apart(
-            {logits_of(a, size), legal_of(a), per_row("actions", actions, a, wide ? 8 : 4),
-             per_row("entropy", g_entropy ? entropy : nullptr, a, 4), per_row("stats", stats, a, 8),
-             per_row("top_action", top_action, a, int64_t{8} * top),
-             strided("g_logprob", g_logprob, a, g_logprob_stride),
-             strided("g_entropy", g_entropy, a, g_entropy_stride),
-             per_row("g_top", g_top, a, int64_t{4} * top), matrix("grad", grad, a, grad_ld, a.v, size, true)}))
+    if (const int rc = check_buffers(
+            {logits_of(a, size), legal_of(a), per_row("actions", actions, a, wide ? 8 : 4, 1),
+             per_row("entropy", g_entropy ? entropy : nullptr, a, 4, 1), per_row("stats", stats, a, 4, 2),
+             per_row("top_action", top_action, a, 8, top), strided("g_logprob", g_logprob, a, g_logprob_stride),
+             strided("g_entropy", g_entropy, a, g_entropy_stride), per_row("g_top", g_top, a, 4, top),
+             result(matrix("grad", grad, a, grad_ld, a.v, size))}))
       return rc;
     const Plan p = grad_plan(a, size);
     const LogprobGradArgs g{actions,    wide != 0,        top,       entropy,          stats,
@@ -375,12 +381,12 @@ int os_az_distill_async(const os_az_rows* rows, const os_az_target* target, cons
     const int64_t need = workspace_bytes_of(a, p, 0);
     const bool parts = need > 0;
     if (const int rc = check_workspace(need, workspace, workspace_bytes)) return rc;
-    if (const int rc = check_apart(
+    if (const int rc = check_buffers(
             {logits_of(a, size), legal_of(a), ids_of(a, t), values_of(a, t),
-             per_row("weight", grad ? weight : nullptr, a, 4), per_row("loss", loss, a, 4, true),
-             per_row("target_entropy", target_entropy, a, 4, true), per_row("stats", stats, a, 8, true),
-             matrix("grad", grad, a, grad_ld, a.v, size, true),
-             Buffer{"workspace", workspace, 1, 0, need, true}}))
+             per_row("weight", grad ? weight : nullptr, a, 4, 1), result(per_row("loss", loss, a, 4, 1)),
+             result(per_row("target_entropy", target_entropy, a, 4, 1)),
+             result(per_row("stats", stats, a, 4, 2)), result(matrix("grad", grad, a, grad_ld, a.v, size)),
+             workspace_of(workspace, need)}))
       return rc;
     DistillArgs g{t, weight, 1, loss, target_entropy, stats, grad, grad_ld, 0};
     return by_dtype(rows->dtype, [&](auto k) {
@@ -418,10 +424,10 @@ int os_az_distill_grad_async(const os_az_rows* rows, const os_az_target* target,
     if (a.n == 0) return OS_OK;
     if (!stats || !grad) return Fail(OS_ERR_INVALID, "null gradient buffer");
     const int size = type_size(rows->dtype);
-    if (const int rc = check_apart({logits_of(a, size), legal_of(a), ids_of(a, t), values_of(a, t),
-                                    strided("weight", weight, a, weight_stride),
-                                    per_row("stats", stats, a, 8),
-                                    matrix("grad", grad, a, grad_ld, a.v, size, true)}))
+    if (const int rc = check_buffers({logits_of(a, size), legal_of(a), ids_of(a, t), values_of(a, t),
+                                      strided("weight", weight, a, weight_stride),
+                                      per_row("stats", stats, a, 4, 2),
+                                      result(matrix("grad", grad, a, grad_ld, a.v, size))}))
       return rc;
     const Plan p = grad_plan(a, size);
     DistillArgs g{t, weight, weight_stride, nullptr, nullptr, const_cast<float*>(stats),

@@ -294,3 +294,51 @@ def test_gpu_written_tensors_change_their_version(require_gpu):
   policy.distill_into(x, t, weight=w, **ds)
   want, tol = ref.distill(x.cpu(), t.cpu())
   close(ds["loss"], want["loss"], tol["loss"], "loss")
+
+
+def test_abi_refuses_misaligned_buffers():
+  """Each operand and result lies at a multiple of its element's size (values that
+  are read for a whole row at once come through the scalar unit, which drops an
+  address's low bits), or the call is refused before any launch."""
+  import ctypes
+  from os_amd import _lib
+  L = _lib.lib
+  n, v, k, top = 4, 9, 3, 2
+  size = dict(actions=8, logprob=4, entropy=4, stats=4, top_action=8, top_logprob=4, g_logprob=4,
+              g_entropy=4, g_top=4, ids=8, target=4, weight=4, loss=4, target_entropy=4)
+
+  def call(name, p, wide, type_):
+    rows = ctypes.byref(_lib.AzRows(logits=p["logits"], num_rows=n, ld=v, num_actions=v, dtype=0,
+                                    temperature=1.0))
+    tg = ctypes.byref(_lib.AzTarget(actions=p["ids"], target=p["target"], actions_ld=k, target_ld=k,
+                                    k=k, type=type_, wide=wide))
+    if name == "logprobs":
+      return L.os_az_logprobs_async(rows, p["actions"], wide, p["logprob"], p["entropy"], p["stats"],
+                                    top, p["top_action"], p["top_logprob"], None, 0, None)
+    if name == "logprobs_grad":
+      return L.os_az_logprobs_grad_async(rows, p["actions"], wide, p["entropy"], p["stats"], top,
+                                         p["top_action"], p["g_logprob"], 1, p["g_entropy"], 1,
+                                         p["g_top"], p["grad"], v, None)
+    if name == "distill":
+      return L.os_az_distill_async(rows, tg, p["weight"], p["loss"], p["target_entropy"], p["stats"],
+                                   p["grad"], v, None, 0, None)
+    return L.os_az_distill_grad_async(rows, tg, p["weight"], 1, p["stats"], p["grad"], v, None)
+  used = dict(logprobs="actions logprob entropy stats top_action top_logprob",
+              logprobs_grad="actions entropy stats top_action g_logprob g_entropy g_top",
+              distill="ids target weight loss target_entropy stats",
+              distill_grad="ids target weight stats")
+  names = ["logits", "grad"] + sorted(size)
+  for name, keys in used.items():
+    for key in keys.split():
+      for wide in (0, 1):
+        for type_ in (_lib.AZ_LOGITS_F32, _lib.AZ_LOGITS_BF16, _lib.AZ_LOGITS_F16, _lib.AZ_WEIGHTS_F32,
+                      _lib.AZ_WEIGHTS_I32):
+          step = size[key]
+          if key in ("actions", "ids") and not wide:
+            step = 4
+          if key == "target" and type_ in (_lib.AZ_LOGITS_BF16, _lib.AZ_LOGITS_F16):
+            step = 2
+          p = {x: 4096 * (1 + i) for i, x in enumerate(names)}
+          p[key] += step // 2
+          assert call(name, p, wide, type_) == _lib.OS_ERR_INVALID, (name, key, wide, type_)
+          assert b"aligned" in L.os_last_error(), (name, key, wide, type_, L.os_last_error())
