@@ -373,8 +373,8 @@ int os_az_mlp_heads_async(const float* obs, int64_t num_rows, int32_t obs_size,
  * with an operand is refused (disjoint columns of one buffer's rows share
  * none), and so is a pointer that is not aligned to its elements.  Every call
  * launches on hip_stream, whose device must be current, allocates nothing and may
- * be captured; it reads no device data on the host, so
- * what ids hold is checked on the device, as said with each. */
+ * be captured; it reads no device data on the host, so what ids hold is checked
+ * on the device, as said with each. */
 #define OS_AZ_F32 0
 #define OS_AZ_BF16 1
 #define OS_AZ_F16 2

@@ -254,9 +254,10 @@ __device__ __forceinline__ float logit(const Rows& a, int64_t r, int64_t i) {
   return a.legal != nullptr && a.legal[r * a.lld + i] == 0 ? neg_inf() : x;
 }
 
-// ln p of a logit: right for any x of the type ((x - m) c may overflow).
+// ln p of a logit: right for any x of the type ((x - m) c may overflow, and x - m
+// where the temperature brings it back: hence the halves).
 __device__ __forceinline__ float log_p(const Rows& a, float x, float m, float l) {
-  return fmaf(x - m, a.inv_t, -l * kLn2);
+  return fmaf(0.5f * x - 0.5f * m, 2.0f * a.inv_t, -l * kLn2);
 }
 
 // The largest of a chunk's values: v_maximum3_f32, which needs no quieting of

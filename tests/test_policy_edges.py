@@ -6,7 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 import policy_ref as ref
-from test_policy import TYPES, close, cuda, make, make_target
+from test_policy import TYPES, check_distill, check_logprobs, close, make
 
 gpu = pytest.mark.gpu
 
@@ -342,3 +342,23 @@ def test_abi_refuses_misaligned_buffers():
           p[key] += step // 2
           assert call(name, p, wide, type_) == _lib.OS_ERR_INVALID, (name, key, wide, type_)
           assert b"aligned" in L.os_last_error(), (name, key, wide, type_, L.os_last_error())
+
+
+@gpu
+@pytest.mark.parametrize("v", [2, 9, 82, 700, 3000, 40000, 150001])
+def test_gpu_logits_at_both_ends_of_the_type(require_gpu, v):
+  """x - m beyond the type's range at a temperature that brings it back in: the log
+  probability is finite."""
+  from os_amd import policy
+  n, t = 3, 4.0
+  big = torch.finfo(torch.float32).max
+  logits = torch.zeros(n, v)
+  logits[:, 0] = torch.tensor([big, 0.9 * big, 0.6 * big])
+  logits[:, v - 1] = torch.tensor([-big, -0.9 * big, -0.7 * big])
+  actions = torch.full((n,), v - 1)
+  check_logprobs(logits, None, actions, 2, t)
+  want, _ = ref.logprobs(logits, actions, None, 0, t)
+  assert bool(torch.isfinite(want["logprob"]).all())
+  ids = torch.tensor([[0, v - 1]] * n)
+  w = torch.tensor([[1.0, 1.0]] * n)
+  check_distill(logits, None, w, ids, "weights", t)
