@@ -6,7 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 import policy_ref as ref
-from test_policy import TYPES, check_distill, check_logprobs, close, make
+from test_policy import TYPES, check_distill, check_logprobs, close, cuda, make, make_target
 
 gpu = pytest.mark.gpu
 
@@ -362,3 +362,59 @@ def test_gpu_logits_at_both_ends_of_the_type(require_gpu, v):
   ids = torch.tensor([[0, v - 1]] * n)
   w = torch.tensor([[1.0, 1.0]] * n)
   check_distill(logits, None, w, ids, "weights", t)
+
+
+# ---- every size of kernel ----
+
+# Rows of up to 64 actions share a wave, of up to 2048 have one that holds 0.5,
+# 1, 1.5, 2, 3, 4, 6 or 8 KiB, longer ones have a workgroup: both sides of each
+# border, in actions of 4 bytes (and of 2: up to 2048 actions, 4 KiB), and sizes
+# whose last chunk is nearly empty or nearly full.
+BORDERS = sorted({b // size + d for b in (512, 1024, 1536, 2048, 3072, 4096, 6144, 8192)
+                  for size in (2, 4) for d in (-1, 0, 1) if b // size + d <= 2049} | {63, 64, 65, 67, 2050})
+
+
+@gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("v", BORDERS)
+def test_gpu_every_operation_at_the_kernels_borders(require_gpu, v, dtype, masked):
+  from os_amd import policy
+  n = 7
+  logits, legal, actions = make(n, v, dtype, masked, 1 if v % 2 else 0, seed=v)
+  # the last action is the likeliest, the given one, or excluded
+  logits[1, v - 1] = 20.0
+  actions[2] = v - 1
+  logits[4, v - 1] = -math.inf
+  if masked:
+    legal[1, v - 1] = legal[2, v - 1] = 1
+    legal[5, v - 1] = 0
+  check_logprobs(logits, legal, actions, 0, 0.7)
+  check_logprobs(logits, legal, actions, 9)
+  g = torch.Generator().manual_seed(v)
+  gl, gh, gt = torch.randn(n, generator=g), torch.randn(n, generator=g), torch.randn(n, 9, generator=g)
+  for top in (0, 9):
+    leaf = cuda(logits).requires_grad_()
+    r = policy.logprobs(leaf, actions.cuda(), cuda(legal), top=top, temperature=1.3)
+    outs, ups = [r.logprob, r.entropy], [gl.cuda(), gh.cuda()]
+    if top:
+      outs.append(r.top_logprob)
+      ups.append(gt.cuda())
+    grad, = torch.autograd.grad(outs, leaf, ups)
+    want, tol = ref.logprobs_grad(logits, actions, legal, 1.3, gl, gh,
+                                  r.top_action.cpu() if top else None, gt if top else None)
+    close(grad, want, tol + ref.rounding(grad.dtype, want), "grad")
+  weight = torch.randn(n, generator=g)
+  k = min(v, 70)
+  target, ids = make_target(n, v, k, legal, "weights", "i32")
+  ids[1, 0] = torch.where(ids[1, 0] < 0, -1, v - 1)
+  ids[1, 1:] = torch.where(ids[1, 1:] == v - 1, -1, ids[1, 1:])
+  check_distill(logits, legal, target, ids, "weights", 1.0, weight, wide=False)
+  ids[3, -1] = ids[3, 0]
+  check_distill(logits, legal, target.float(), ids, "weights", 0.8, weight)
+  if v <= 1024:
+    target, _ = make_target(n, v, v, legal, "logits", dtype, dense=True)
+    if masked:
+      target = target.masked_fill(legal == 0, -math.inf)
+    target[4, v - 1] = -math.inf
+    check_distill(logits, legal, target, None, "logits", 1.5, weight)
