@@ -418,3 +418,86 @@ def test_gpu_every_operation_at_the_kernels_borders(require_gpu, v, dtype, maske
       target = target.masked_fill(legal == 0, -math.inf)
     target[4, v - 1] = -math.inf
     check_distill(logits, legal, target, None, "logits", 1.5, weight)
+
+
+# ---- float32 arithmetic, held to what it can do ----
+
+def _roundings(v):
+  """Roundings that a sum over a row of v float32 actions meets, at most.  Up to 64
+  actions: four a lane, four steps over 16 lanes.  Up to 2048: the lane's elements
+  one after the other (as many as the kernel holds), six steps, three more for the
+  quotient by the maximum's own exponential.  Longer rows: four in a chunk, then up
+  to 8 chunks (where rows are few; a product, a sum and two for the factor each), then
+  lanes, waves and parts (6, 4 and 6 steps), four roundings for each of the three
+  changes of the reference."""
+  if v <= 64:
+    return 8
+  if v <= 2048:
+    return 2 * min(u for u in (1, 2, 3, 4, 6, 8, 12, 16) if u * 128 >= v) + 6 + 3
+  return 4 + 8 * 4 + 6 + 4 + 6 + 12 + 3
+
+
+def _row_sizes(x):
+  """p, log p, the distances to the maximum (nats) and their mean under p."""
+  p, logp = ref.softmax(x)
+  d = torch.where(p > 0, x.amax(1, keepdim=True) - x, torch.zeros_like(x))
+  return p, logp, d, (p * d).sum(1)
+
+
+@gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("v", [7, 64, 82, 362, 768, 1025, 2047, 4099, 20011, 32769, 70001, 131072])
+def test_gpu_float32_precision(require_gpu, v, masked):
+  """An exponential is off by an ulp (two half steps U) and by its argument's two
+  roundings, 2 U a nat of distance d from the maximum (3 U where chunks were
+  rescaled).  With R roundings in the sum, s is off by U (R + 2 + 3 E d), E under p;
+  the logarithm of s by that, and 2 U of itself.  p = e / s in the gradient has
+  U (R + 2 + 3 E d + 2 + 3 d + 3 log s + 6): the exponentials of d and of log s, and
+  three products.  The entropy is log s + E d: an exponential's error e acts as
+  p |log p + H| e on it, the two sums' R as U R (1 + 2 E d), the terms' products and
+  the quotient as 4 U E d.  (Statistics of 11 bits, half a step of 2^-12, would be off
+  by ten times these bounds and more.)"""
+  from os_amd import policy
+  n, t = 5, 0.8
+  logits, legal, actions = make(n, v, "f32", masked, 0, seed=77)
+  actions = torch.arange(n) * 31 % v
+  if masked:
+    legal[torch.arange(n), actions] = 1
+  x = ref.masked(logits, legal, t)
+  p, logp, d, mean = _row_sizes(x)
+  logs = -(logp + d).amax(1)  # log p of the maximum, but for its sign
+  logs = torch.where(torch.isfinite(logs), logs, torch.zeros_like(logs)).abs()
+  R = _roundings(v)
+  s_err = R + 2 + 3 * mean + 2 * logs
+  assert float((s_err + 8 + 3 * logs).max()) * ref.U < 2.0 ** -12 / 10
+  leaf = logits.cuda().requires_grad_()
+  r = policy.logprobs(leaf, actions.cuda(), None if legal is None else legal.cuda(), temperature=t)
+  entropy = -ref.plogp(p, logp).sum(1)
+  own = torch.where(p > 0, p * (logp + entropy[:, None]).abs() * (2 + 3 * d), torch.zeros_like(p))
+  h_err = R * (1 + 2 * mean) + own.sum(1) + 4 * mean + 2 * logs + entropy.abs() + 4
+  close(r.entropy, entropy, ref.U * h_err, "entropy")
+  at = actions[:, None]
+  lp = logp.gather(1, at)[:, 0]
+  close(r.logprob, lp, ref.U * (s_err + 4 * d.gather(1, at)[:, 0] + lp.abs() + 2), "logprob")
+  # a log probability's gradient, p's relative error apart from the given action's 1
+  one = torch.ones(n)
+  grad, = torch.autograd.grad(r.logprob, leaf, one.cuda(), retain_graph=True)
+  hot = torch.zeros(n, v, dtype=torch.float64).scatter_(1, at, 1.0)
+  rel = (s_err + 8)[:, None] + 3 * d + 3 * logs[:, None]
+  want = torch.where(x > -math.inf, hot - p, torch.zeros_like(p)) / t
+  tol = torch.where(x > -math.inf, ref.U * (p * rel + 3 * hot) + ref.LEAST, torch.zeros_like(p)) / t
+  close(grad, want, tol + ref.rounding(torch.float32, want), "logprob gradient")
+  # cross entropy on that action: the same with the other sign
+  both, loss = torch.empty_like(leaf), torch.empty(n, device="cuda")
+  policy.distill_into(leaf.detach(), one[:, None].cuda(), loss, None, at.cuda(),
+                      None if legal is None else legal.cuda(), temperature=t, grad=both)
+  close(both, -want, tol + ref.rounding(torch.float32, want), "loss gradient")
+  close(loss, -lp, ref.U * (s_err + 4 * d.gather(1, at)[:, 0] + 3 * lp.abs() + 2), "loss")
+  # the entropy's gradient: -p (log p + H), the parts' errors on top of p's
+  grad, = torch.autograd.grad(r.entropy, leaf, one.cuda())
+  h = entropy[:, None]
+  want = torch.where(p > 0, -p * (logp + h), torch.zeros_like(p)) / t
+  size = torch.where(p > 0, p * (logp.abs() + h + d + logs[:, None] + 1), torch.zeros_like(p))
+  tol = torch.where(x > -math.inf, ref.U * (size * (rel + 4) + p * h_err[:, None]) + ref.LEAST * (105 + h),
+                    torch.zeros_like(p)) / t
+  close(grad, want, tol + ref.rounding(torch.float32, want), "entropy gradient")
