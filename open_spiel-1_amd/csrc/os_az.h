@@ -134,6 +134,19 @@ OS_HD void az_request(const GameCfg& g, const typename G::State& s, int kind, co
   for (int k = 0; k < l.count; ++k) io.legal[l.kth(k)] = 1;
 }
 
+// Lanes leave az_step's loops at different rounds, each for a reason of its own.
+// The reason is an integer that the compiler cannot see through, and every loop
+// has one exit: with returns and breaks of their own, the exits become lane masks
+// that are merged over the rounds, and hipcc 7.2 took such a mask, spilled, for
+// undefined at the head of each round (k_az_step<Hex> built without packed float32
+// operations: a lane that had left to ask for a prior was counted as finished).
+OS_HD int az_opaque(int x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(x));
+#endif
+  return x;
+}
+
 // Advances one search until it needs the evaluator (request written, returns)
 // or finishes (kind = kAzNone, stage = kAzDone).  `ctx` is the game's
 // history context with its root fields set (go: Zobrist table, the positions
@@ -154,10 +167,12 @@ OS_HD void az_step(const GameCfg& g, const SearchParams& sp, int puct,
   const double inf = __builtin_huge_val();
   typename G::State s = sl.s;
   int depth = sl.depth;
-  int phase;  // 0 new simulation, 1 descend, 2 expand with priors, 3 value ready
+  // 0 new simulation, 1 descend, 2 expand with priors, 3 value ready, 4 expand with
+  // the parked priors of a fused request
+  int phase;
+  int ask = kAzNone;  // the request to leave with (kAzNone: finished)
   double v0 = 0.0;
   bool solved = false;
-  bool from_raw = false;  // phase 2 takes the parked priors of a fused request
   if (sl.stage == kAzDone) {
     *io.kind = kAzNone;
     return;
@@ -199,17 +214,22 @@ OS_HD void az_step(const GameCfg& g, const SearchParams& sp, int puct,
       }
     }
   }
-  for (;;) {
-    if (phase < 0) break;
+  int run = az_opaque(phase >= 0);
+  while (run != 0) {
+    int stop = 0;
     if (phase == 0) {
-      if (sl.sim >= sp.max_simulations) break;
-      s = root;
-      ctx.reset();
-      depth = 0;
-      sl.path[0] = 0;
-      phase = 1;
+      if (sl.sim >= sp.max_simulations) {
+        stop = 1;
+      } else {
+        s = root;
+        ctx.reset();
+        depth = 0;
+        sl.path[0] = 0;
+        phase = 1;
+      }
     }
-    if (phase == 2) {
+    if (phase == 2 || phase == 4) {
+      const bool from_raw = phase == 4;
       // Prior of the pending node (legal order), shuffled with the bot rng
       // like std::shuffle over (action, prior) pairs (mcts.cc:275-282).
       const uint32_t x = sl.path[depth];
@@ -217,55 +237,50 @@ OS_HD void az_step(const GameCfg& g, const SearchParams& sp, int puct,
       const int nc = l.count;
       if (!from_raw && sl.used + static_cast<uint32_t>(nc) > cap) {
         sl.res.status = kArenaOverflow;
-        break;
+        stop = 1;
+        phase = 0;
+      } else {
+        const bool noisy = x == 0 && nz.noise != nullptr;
+        if (noisy)  // dirichlet_noise consumed these words of rng_ (mcts.cc:265-267)
+          for (int i = 0; i < nz.skip; ++i) bot.next();
+        uint8_t perm[kMaxChildren];
+        for (int k = 0; k < nc; ++k) perm[k] = static_cast<uint8_t>(k);
+        if (np_policy) NpShuffle(perm, nc, bot);  // mcts.py:320
+        else CppShuffle(perm, nc, bot);
+        const uint32_t first = from_raw ? nodes[x].first : sl.used;
+        for (int k = 0; k < nc; ++k) {
+          const int j = perm[k];
+          const int a = l.kth(j);
+          const double p = from_raw ? raw[first + j] : io.prior[a];
+          Node<double>& c = nodes[first + k];
+          c.first = 0;
+          c.n = 0;
+          c.w = 0.0;
+          c.action = static_cast<uint16_t>(a);
+          c.nchild = 0;
+          c.out = kUnsolved;
+          // (1 - eps) * p + eps * noise, separately rounded (mcts.cc:269-271)
+          prior[first + k] = noisy ? (1.0 - nz.eps) * p + nz.eps * nz.noise[j] : p;
+        }
+        nodes[x].first = first;
+        nodes[x].nchild = static_cast<uint8_t>(nc);
+        if (!from_raw) sl.used += nc;
+        sl.nodes_count += nc;
+        sl.res.expanded += nc;
+        phase = 1;
       }
-      const bool noisy = x == 0 && nz.noise != nullptr;
-      if (noisy)  // dirichlet_noise consumed these words of rng_ (mcts.cc:265-267)
-        for (int i = 0; i < nz.skip; ++i) bot.next();
-      uint8_t perm[kMaxChildren];
-      for (int k = 0; k < nc; ++k) perm[k] = static_cast<uint8_t>(k);
-      if (np_policy) NpShuffle(perm, nc, bot);  // mcts.py:320
-      else CppShuffle(perm, nc, bot);
-      const uint32_t first = from_raw ? nodes[x].first : sl.used;
-      for (int k = 0; k < nc; ++k) {
-        const int j = perm[k];
-        const int a = l.kth(j);
-        const double p = from_raw ? raw[first + j] : io.prior[a];
-        Node<double>& c = nodes[first + k];
-        c.first = 0;
-        c.n = 0;
-        c.w = 0.0;
-        c.action = static_cast<uint16_t>(a);
-        c.nchild = 0;
-        c.out = kUnsolved;
-        // (1 - eps) * p + eps * noise, separately rounded (mcts.cc:269-271)
-        prior[first + k] = noisy ? (1.0 - nz.eps) * p + nz.eps * nz.noise[j] : p;
-      }
-      nodes[x].first = first;
-      nodes[x].nchild = static_cast<uint8_t>(nc);
-      if (!from_raw) sl.used += nc;
-      from_raw = false;
-      sl.nodes_count += nc;
-      sl.res.expanded += nc;
-      phase = 1;
     }
     if (phase == 1) {
-      for (;;) {
+      enum : int { kDeeper, kLeaf, kRaw, kAsk, kTooDeep };
+      int at = kDeeper;
+      while (at == kDeeper) {
         const uint32_t x = sl.path[depth];
         const Node<double> nx = nodes[x];
-        if (G::terminal(s, g) || nx.n <= 0) break;
-        if (nx.nchild == 0 && raw != nullptr && nx.first != 0) {
-          from_raw = true;  // parked by this node's fused request: expand now
-          break;
-        }
-        if (nx.nchild == 0) {
-          sl.s = s;
-          sl.depth = depth;
-          az_save_log(ctx, sl.glog);
-          sl.stage = kAzWaitPrior;
-          az_request<G>(g, s, kAzPrior, io, obs_size, num_actions, ctx);
-          return;
-        }
+        int end = kDeeper;
+        if (G::terminal(s, g) || nx.n <= 0) end = kLeaf;
+        else if (nx.nchild == 0) end = raw != nullptr && nx.first != 0 ? kRaw : kAsk;
+        at = az_opaque(end);
+        if (at != kDeeper) continue;
         const int cp = P0 ^ (depth & 1);
         const double dN = static_cast<double>(nx.n);
         const double logN = sp.log_lut[nx.n];
@@ -296,30 +311,30 @@ OS_HD void az_step(const GameCfg& g, const SearchParams& sp, int puct,
         G::apply(s, g, ctx, nodes[ci].action);
         if (++depth >= kMaxPath) {
           sl.res.status = kPathOverflow;
-          sl.stage = kAzDone;
-          *io.kind = kAzNone;
-          return;
+          at = az_opaque(kTooDeep);
+        } else {
+          sl.path[depth] = ci;
         }
-        sl.path[depth] = ci;
       }
-      if (from_raw) {
-        phase = 2;
-        continue;
-      }
-      if (depth > sl.res.max_depth) sl.res.max_depth = depth;
-      if (G::terminal(s, g)) {
-        const int r0 = G::ret0(s, g, ctx);
-        nodes[sl.path[depth]].out = static_cast<int8_t>(r0);
-        solved = sp.solve != 0;
-        v0 = static_cast<double>(r0);
-        phase = 3;
+      if (at == kRaw) {  // parked by this node's fused request: expand now
+        phase = 4;
+      } else if (at == kAsk) {
+        ask = kAzPrior;
+        stop = 1;
+      } else if (at == kTooDeep) {
+        stop = 1;
       } else {
-        sl.s = s;
-        sl.depth = depth;
-        az_save_log(ctx, sl.glog);
-        sl.stage = kAzWaitValue;
-        az_request<G>(g, s, raw != nullptr ? kAzBoth : kAzValue, io, obs_size, num_actions, ctx);
-        return;
+        if (depth > sl.res.max_depth) sl.res.max_depth = depth;
+        if (G::terminal(s, g)) {
+          const int r0 = G::ret0(s, g, ctx);
+          nodes[sl.path[depth]].out = static_cast<int8_t>(r0);
+          solved = sp.solve != 0;
+          v0 = static_cast<double>(r0);
+          phase = 3;
+        } else {
+          ask = raw != nullptr ? kAzBoth : kAzValue;
+          stop = 1;
+        }
       }
     }
     if (phase == 3) {
@@ -356,21 +371,34 @@ OS_HD void az_step(const GameCfg& g, const SearchParams& sp, int puct,
       }
       sl.sim += 1;
       sl.res.sims = sl.sim;
-      if (nodes[0].out != kUnsolved) break;  // mcts.cc:398-401, mcts.py:440-441
-      if (!np_policy && nodes[0].nchild == 1) break;
-      if (sp.max_nodes > 1 && sl.nodes_count >= sp.max_nodes) {      // mcts.cc:402-424
+      if (nodes[0].out != kUnsolved) {  // mcts.cc:398-401, mcts.py:440-441
+        stop = 1;
+      } else if (!np_policy && nodes[0].nchild == 1) {
+        stop = 1;
+      } else if (sp.max_nodes > 1 && sl.nodes_count >= sp.max_nodes) {  // mcts.cc:402-424
         const int st = garbage_collect(nodes, sl.used, cap, sl.gc_limit, &sl.nodes_count);
         if (st != kOk) {
           sl.res.status = st;
-          break;
+          stop = 1;
+        } else {
+          sl.res.gc_runs++;
+          sl.gc_limit = static_cast<int>(sl.gc_limit *
+                                         (sl.nodes_count > sp.max_nodes / 2 ? 1.25 : 0.9));
+          if (sl.gc_limit < 5) sl.gc_limit = 5;
         }
-        sl.res.gc_runs++;
-        sl.gc_limit = static_cast<int>(sl.gc_limit *
-                                       (sl.nodes_count > sp.max_nodes / 2 ? 1.25 : 0.9));
-        if (sl.gc_limit < 5) sl.gc_limit = 5;
       }
       phase = 0;
     }
+    run = az_opaque(stop == 0);
+  }
+  ask = az_opaque(ask);
+  if (ask != kAzNone) {
+    sl.s = s;
+    sl.depth = depth;
+    az_save_log(ctx, sl.glog);
+    sl.stage = ask == kAzPrior ? kAzWaitPrior : kAzWaitValue;
+    az_request<G>(g, s, ask, io, obs_size, num_actions, ctx);
+    return;
   }
   sl.res.nodes = sl.nodes_count;
   sl.res.used = sl.used;
