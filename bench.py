@@ -31,6 +31,7 @@ import argparse
 import hashlib
 import json
 import os
+import re
 import socket
 import subprocess
 import sys
@@ -1173,21 +1174,25 @@ def cpu_baseline_playouts(game, seconds):
 
 
 # Host-side units: the C-ABI, batch preparation and the small reduction
-# kernels (k_root_*, k_outcome_counts, k_sum_devices); the PMC'd kernels
-# (k_wsearch, k_mcts, k_rollouts, k_az_step, k_wselfplay) do not include them.
-HOST_UNITS = ("os_engine.hip", "os_host.cpp", "os_host.h", "Makefile")
+# kernels (k_root_*, k_outcome_counts, k_sum_devices), and the policy operators
+# (os_policy*); the PMC'd kernels (k_wsearch, k_mcts, k_rollouts, k_az_step,
+# k_wselfplay) do not include them.
+HOST_UNITS = ("os_engine.hip", "os_host.cpp", "os_host.h", "os_error.h")
 
 
 def kernel_source_hash():
-  """sha256 over the sources of the PMC'd kernels (csrc/* minus the host
-  units): ties a PMC record to the code it was collected on
-  (tools/pmc_summary.py stores the same hash)."""
+  """sha256 over the sources of the PMC'd kernels (csrc/* minus the units above)
+  and the flags they are compiled with: ties a PMC record to the code it was
+  collected on (tools/pmc_summary.py stores the same hash)."""
   h = hashlib.sha256()
   src = os.path.join(ROOT, "open_spiel-1_amd", "csrc")
   for name in sorted(os.listdir(src)):
-    if name.endswith((".h", ".hip", ".cpp")) and name not in HOST_UNITS:
+    if (name.endswith((".h", ".hip", ".cpp")) and name not in HOST_UNITS
+        and not name.startswith("os_policy")):
       with open(os.path.join(src, name), "rb") as f:
         h.update(name.encode() + b"\0" + f.read())
+  with open(os.path.join(src, "Makefile")) as f:
+    h.update(re.search(r"^FLAGS :=(.*\\\n)*.*", f.read(), flags=re.M).group(0).encode())
   return h.hexdigest()[:16]
 
 
