@@ -52,4 +52,5 @@ def test_a_counter_record_goes_stale_with_its_kernels_only(tmp_path, monkeypatch
   assert not changed("Makefile", "POLICY := ", "POLICY := x ")
   for name in ("os_wave.h", "os_az.h", "os_kernels.h", "os_game_go.hip"):
     assert changed(name), name
-  assert changed("Makefile", "-O3", "-O2") and changed("Makefile", "-packed-fp32-ops", "-x")
+  assert changed("Makefile", "-O3 -std", "-O2 -std")
+  assert changed("Makefile", "-Xclang -packed-fp32-ops ", "")
