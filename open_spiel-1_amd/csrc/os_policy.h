@@ -18,8 +18,8 @@
 // ONCE, by whole workgroups, and stays in registers (16 chunks of 16 bytes a
 // lane: up to 256 KiB a workgroup, the register file being 512 KiB a compute
 // unit) from the sums to the gradient or the selection of the top actions.
-// 2048 rows of 131072 bf16 actions: top 20 in 124 us (4.3 TB/s read), loss and
-// gradient in 242 us (4.4 TB/s read and written; a copy of 2 GiB: 4.9 TB/s).
+// 2048 rows of 131072 bf16 actions: top 20 in 123 us (4.4 TB/s read), loss and
+// gradient in 244 us (4.4 TB/s read and written; a copy of 2 GiB: 4.9 TB/s).
 // Short rows (k_wave) are bound by the vector units, few rows by latency.
 // The maximum and the sums run together over the chunks as they arrive (a
 // running maximum, the sums rescaled by it), and a chunk's registers are
@@ -463,8 +463,8 @@ __device__ __forceinline__ void target_entries(const Target& t, int64_t r, int f
     // weights' z <= 0 case)
     const bool in = (first + i * step < t.k) & (raw[i] >= 0), past = raw[i] >= v;
     const bool none = !in | (is_weights(t) & (z[i] <= 0.0f));
-    bad = in & past ? 1.0f : bad;
-    id[i] = in & !past ? raw[i] : -1;
+    bad = (in & past) ? 1.0f : bad;
+    id[i] = (in & !past) ? raw[i] : -1;
     z[i] = none ? no_mass(t) : z[i];
   });
 }
@@ -528,8 +528,8 @@ struct RawEntries {
         // lost the weights' f <= 0 case)
         const bool in = (first + i * step < t.k) & (a >= 0), past = a >= v;
         const bool none = !in | (is_weights(t) & (f <= 0.0f));
-        bad = in & past ? 1.0f : bad;
-        out[i] = in & !past ? static_cast<int>(a) : -1;
+        bad = (in & past) ? 1.0f : bad;
+        out[i] = (in & !past) ? static_cast<int>(a) : -1;
         value[i] = none ? no_mass(t) : f;
       }
     }
@@ -1357,9 +1357,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
 // next row's chunks are under way while a row is worked on.  No barrier is
 // needed: what goes through LDS stays within the wave, whose accesses are in
 // order (fence() keeps the compiler to it).  The vector units are what a row
-// waits for here, 30 operations an element with the mask and the top actions
-// (65536 x 768 masked bf16, top 8: 52 us, units 73% busy; 32 us is the
-// memory's share), so rows take the smallest kernel that holds them and only the
+// waits for here: 366 instructions a row of 12 actions a lane with the mask and
+// the top actions, a third of them the elements' own, the rest the row's folds,
+// bound, ranking and addresses (65536 x 768 masked bf16, top 8: 52 us, units three
+// quarters busy; 32 us is the memory's share), so rows take the smallest kernel that holds them and only the
 // last chunk is ever short, of six and eight the last two (the same in two chunks
 // of 16 bytes rather than three of 8: 4 us more).  Against a workgroup of k_rows
 // it saves the barriers: 44739 x 1500 f32, top 8: 99 -> 54 us, loss and gradient:
@@ -1443,7 +1444,9 @@ __global__ __launch_bounds__(64, (kWaveRoom<kMask, kWaveEach<T, W, kC>, kOp>)) v
           if (j < drop[t - kFull]) x[t * kE + j] = neg_inf();
       }
     }
-    // -- what else the row needs from memory, ahead of the next row's loads --
+    // -- what else the row needs from memory, issued ahead of the next row's loads
+    // (the given action's logit is waited for at its mask byte, which logit()
+    // branches on; the target's entries where they are used) --
     const RowValues<kOp> val = next;
     const int64_t given = val.given;
     float given_x = neg_inf();

@@ -227,9 +227,10 @@ def _workspace(rows, a, top, dev):
 def logprobs_into(logits, entropy, logprob=None, actions=None, legal=None, top_action=None,
                   top_logprob=None, temperature=1.0, stats=None):
   """logprobs into given tensors: entropy and logprob float32 [N], top_action
-  int64 and top_logprob float32 [N, top], stats float32 [N, 2] (what the
-  gradient needs; optional).  logprob and actions go together, and so do the
-  top pair."""
+  int64 and top_logprob float32 [N, top], stats float32 [N, 2] (what
+  os_az_logprobs_grad_async reads; optional).  logprob and actions go together,
+  and so do the top pair.  What is written may not overlap anything else of the
+  call."""
   rows, n, a, dev = _rows(logits, legal, temperature)
   act, wide = _actions(actions, n, dev)
   if (logprob is None) != (actions is None):
@@ -257,9 +258,10 @@ def logprobs_into(logits, entropy, logprob=None, actions=None, legal=None, top_a
 def distill_into(logits, target, loss, target_entropy=None, target_actions=None, legal=None,
                  kind="weights", temperature=1.0, weight=None, grad=None, stats=None):
   """distill into given tensors: loss and target_entropy float32 [N], stats
-  float32 [N, 2] (what the gradient needs; optional).  With `grad` (the logits'
-  type and shape, any row stride) also the logits' gradient of
-  (weight * loss).sum(); weight float32 [N], None: 1."""
+  float32 [N, 2] (what os_az_distill_grad_async reads; optional).  With `grad`
+  (the logits' type and shape, any row stride) also the logits' gradient of
+  (weight * loss).sum(); weight float32 [N], None: 1.  What is written may not
+  overlap anything else of the call."""
   rows, n, a, dev = _rows(logits, legal, temperature)
   t = _target(target, target_actions, n, a, dev, kind)
   if loss is None:
@@ -436,7 +438,7 @@ def distill(logits, target, target_actions=None, legal=None, kind="weights", tem
   is a weight (kind="weights", float32 or int32: q = w / sum w, weights not
   above 0 count as 0) or a teacher's logit (kind="logits": q =
   softmax(target / temperature) over the row's entries).  Without
-  target_actions the target is [N, A], entry j action j.
+  target_actions the target is [N, A], A <= 1024, entry j action j.
 
   The loss is 0 for a row without a target, +inf where an excluded action has
   mass, NaN where an action >= A is listed.  The gradient reaches the logits,
