@@ -5,7 +5,6 @@
 
 #include <algorithm>
 #include <cstdint>
-#include <initializer_list>
 #include <string>
 
 #include "os_error.h"
@@ -200,7 +199,7 @@ struct Buffer {
   bool out;
 };
 
-// [first, past) of the buffer (a stride so large that it leaves 64 bits: to the end).
+// The end of the buffer (a stride so large that it leaves 64 bits: of the memory).
 uint64_t past(const Buffer& b) {
   uint64_t far, end;
   const uint64_t at = reinterpret_cast<uintptr_t>(b.p);
@@ -210,30 +209,36 @@ uint64_t past(const Buffer& b) {
   return end;
 }
 
-bool overlap(const Buffer& a, const Buffer& b) {
+// Of two buffers whose extents meet: whether they are disjoint columns of one
+// buffer's rows.
+bool columns(const Buffer& a, const Buffer& b) {
+  if (a.ld != b.ld || a.ld == 0) return false;
   const uint64_t a0 = reinterpret_cast<uintptr_t>(a.p), b0 = reinterpret_cast<uintptr_t>(b.p);
-  if (a0 >= past(b) || b0 >= past(a)) return false;
-  if (a.ld != b.ld || a.ld == 0) return true;
-  // fine as disjoint columns of one buffer's rows
   const uint64_t ld = static_cast<uint64_t>(a.ld);
   const uint64_t off = b0 >= a0 ? (b0 - a0) % ld : (ld - (a0 - b0) % ld) % ld;
-  return off < static_cast<uint64_t>(a.bytes) || off + static_cast<uint64_t>(b.bytes) > ld;
+  return off >= static_cast<uint64_t>(a.bytes) && off + static_cast<uint64_t>(b.bytes) <= ld;
 }
 
 // Elements lie at multiples of their size (a row's single values are scalar
 // loads, which drop an address's low bits).  Results share no memory with each
 // other or with what the call reads: rows are worked on in any order, and some
 // operands are read again after a result is written.
-int check_buffers(std::initializer_list<Buffer> all) {
-  const auto there = [](const Buffer& b) { return b.p != nullptr && b.n > 0 && b.bytes > 0; };
-  for (const Buffer* a = all.begin(); a != all.end(); ++a) {
-    if (!there(*a)) continue;
-    if (reinterpret_cast<uintptr_t>(a->p) & static_cast<uintptr_t>(a->size - 1))
-      return Fail(OS_ERR_INVALID, std::string(a->name) + " not aligned to its type");
-    if (!a->out) continue;
-    for (const Buffer* b = all.begin(); b != all.end(); ++b)
-      if (a != b && (!b->out || a < b) && there(*b) && overlap(*a, *b))
-        return Fail(OS_ERR_INVALID, std::string(a->name) + " overlaps " + b->name);
+template <int kCount>
+int check_buffers(const Buffer (&all)[kCount]) {
+  uint64_t lo[kCount], hi[kCount];
+  for (int i = 0; i < kCount; ++i) {
+    const Buffer& a = all[i];
+    const bool there = a.p != nullptr && a.n > 0 && a.bytes > 0;
+    lo[i] = there ? reinterpret_cast<uintptr_t>(a.p) : UINT64_MAX;
+    hi[i] = there ? past(a) : 0;
+    if (there && (lo[i] & static_cast<uint64_t>(a.size - 1)))
+      return Fail(OS_ERR_INVALID, std::string(a.name) + " not aligned to its type");
+  }
+  for (int i = 0; i < kCount; ++i) {
+    if (!all[i].out) continue;
+    for (int j = 0; j < kCount; ++j)
+      if (lo[i] < hi[j] && lo[j] < hi[i] && i != j && !columns(all[i], all[j]))
+        return Fail(OS_ERR_INVALID, std::string(all[i].name) + " overlaps " + all[j].name);
   }
   return OS_OK;
 }

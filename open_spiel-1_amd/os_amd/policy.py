@@ -65,7 +65,9 @@ except AttributeError:
   def _raw_stream(device):
     return torch.cuda.current_stream(device).cuda_stream
 
-try:  # its check of the argument takes three times as long as the rest
+# How autograd learns that a call wrote given tensors: a graph that saved one of
+# them before refuses to run backward.
+try:  # (the public one's check of its argument takes three times as long as the rest)
   _increment_version = torch._C._increment_version
 except AttributeError:
   _increment_version = torch.autograd.graph.increment_version
@@ -204,12 +206,6 @@ def _launch(fn, dev, *args):
     check(rc)
 
 
-def _written(*out):
-  """Autograd learns that a call wrote these (those that there are): a graph that
-  saved one of them before refuses to run backward."""
-  _increment_version([x for x in out if x is not None])
-
-
 def _workspace(rows, a, top, dev):
   """(tensor to keep until the call, address, bytes): rows of few actions need
   none (os_az_rows_workspace)."""
@@ -239,19 +235,24 @@ def logprobs_into(logits, entropy, logprob=None, actions=None, legal=None, top_a
     raise ValueError("top_action and top_logprob go together")
   if entropy is None:
     raise ValueError("entropy is needed")
-  lp = None if logprob is None else _like("logprob", logprob, dev, _F32, n)
-  st = None if stats is None else _like("stats", stats, dev, _F32, n, 2)
-  top, ta, tl = 0, None, None
+  written, lp, st, top, ta, tl = [entropy], None, None, 0, None, None
+  if logprob is not None:
+    lp = _like("logprob", logprob, dev, _F32, n)
+    written.append(logprob)
+  if stats is not None:
+    st = _like("stats", stats, dev, _F32, n, 2)
+    written.append(stats)
   if top_action is not None:
     if top_action.dim() != 2 or top_action.shape[1] > _lib.AZ_MAX_TOP:
       raise ValueError("top_action must be [N, top], top <= %d" % _lib.AZ_MAX_TOP)
     top = top_action.shape[1]
     ta = _like("top_action", top_action, dev, torch.int64, n, top)
     tl = _like("top_logprob", top_logprob, dev, _F32, n, top)
+    written += (top_action, top_logprob)
   h = _like("entropy", entropy, dev, _F32, n)
   keep, work, size = _workspace(rows, a, top, dev)
   _launch(lib.os_az_logprobs_async, dev, rows, act, wide, lp, h, st, top, ta, tl, work, size)
-  _written(entropy, logprob, stats, top_action, top_logprob)
+  _increment_version(written)
   del keep
 
 
@@ -268,14 +269,21 @@ def distill_into(logits, target, loss, target_entropy=None, target_actions=None,
     raise ValueError("loss is needed")
   if weight is not None and grad is None:
     raise ValueError("weight scales the gradient: it needs grad")
-  g, ld = (None, 0) if grad is None else _grad_buffer(grad, logits, n, a, dev)
+  written, g, ld, h, st = [loss], None, 0, None, None
+  if grad is not None:
+    g, ld = _grad_buffer(grad, logits, n, a, dev)
+    written.append(grad)
   w = None if weight is None else _like("weight", weight, dev, _F32, n)
   out = _like("loss", loss, dev, _F32, n)
-  h = None if target_entropy is None else _like("target_entropy", target_entropy, dev, _F32, n)
-  st = None if stats is None else _like("stats", stats, dev, _F32, n, 2)
+  if target_entropy is not None:
+    h = _like("target_entropy", target_entropy, dev, _F32, n)
+    written.append(target_entropy)
+  if stats is not None:
+    st = _like("stats", stats, dev, _F32, n, 2)
+    written.append(stats)
   keep, work, size = _workspace(rows, a, 0, dev)
   _launch(lib.os_az_distill_async, dev, rows, t, w, out, h, st, g, ld, work, size)
-  _written(loss, target_entropy, stats, grad)
+  _increment_version(written)
   del keep
 
 
