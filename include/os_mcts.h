@@ -449,9 +449,9 @@ int os_az_logprobs_grad_async(const os_az_rows* rows, const void* actions, int32
  * listed (NULL: not wanted; where a row's actions are distinct, loss -
  * target_entropy is the Kullback-Leibler divergence from the target; an action
  * listed more than once adds the entropy of its split into entries), stats as
- * above (NULL: not wanted).  grad != NULL: grad[r][i] = weight[r] d loss[r] / d logits[r][i]
- * = weight[r] (p_i sum q - q_i) / temperature, 0 where the action is excluded;
- * weight NULL: 1. */
+ * above (NULL: not wanted).  grad != NULL: grad[r][i] = weight[r] d loss[r] /
+ * d logits[r][i] = weight[r] (p_i sum q - q_i) / temperature, 0 where the action is
+ * excluded; weight NULL: 1. */
 int os_az_distill_async(const os_az_rows* rows, const os_az_target* target,
                             const float* weight, float* loss, float* target_entropy,
                             float* stats, void* grad, int64_t grad_ld, void* workspace,

@@ -1360,11 +1360,11 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_rows(Rows a, Parts pt, ArgsO
 // waits for here: 366 instructions a row of 12 actions a lane with the mask and
 // the top actions, a third of them the elements' own, the rest the row's folds,
 // bound, ranking and addresses (65536 x 768 masked bf16, top 8: 52 us, units three
-// quarters busy; 32 us is the memory's share), so rows take the smallest kernel that holds them and only the
-// last chunk is ever short, of six and eight the last two (the same in two chunks
-// of 16 bytes rather than three of 8: 4 us more).  Against a workgroup of k_rows
-// it saves the barriers: 44739 x 1500 f32, top 8: 99 -> 54 us, loss and gradient:
-// 152 -> 115 us.
+// quarters busy; 32 us is the memory's share), so rows take the smallest kernel
+// that holds them and only the last chunk is ever short, of six and eight the last
+// two (the same in two chunks of 16 bytes rather than three of 8: 4 us more).
+// Against a workgroup of k_rows it saves the barriers: 44739 x 1500 f32, top 8: 99
+// -> 54 us, loss and gradient: 152 -> 115 us.
 // Waves a SIMD that the registers must leave room for (left alone, the compiler
 // keeps every address it could compute again): what the dependent steps of a row
 // leave idle, other rows fill (8 rather than 7 at that size: 57 -> 53 us).
