@@ -370,8 +370,8 @@ def test_gpu_logits_at_both_ends_of_the_type(require_gpu, v):
 # 1, 1.5, 2, 3, 4, 6 or 8 KiB, longer ones have a workgroup: both sides of each
 # border, in actions of 4 bytes (and of 2: up to 2048 actions, 4 KiB), and sizes
 # whose last chunk is nearly empty or nearly full.
-BORDERS = sorted({b // size + d for b in (512, 1024, 1536, 2048, 3072, 4096, 6144, 8192)
-                  for size in (2, 4) for d in (-1, 0, 1) if b // size + d <= 2049} | {63, 64, 65, 67, 2050})
+BORDERS = sorted({512 * b // size + d for b in (1, 2, 3, 4, 6, 8, 12, 16) for size in (2, 4)
+                  for d in (-1, 0, 1) if 512 * b // size + d <= 2049} | {63, 64, 65, 67, 2050})
 
 
 @gpu
